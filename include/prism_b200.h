@@ -298,6 +298,96 @@ int prism_b200_gemm_bf16_fill_plan(int tiles, int pairs, int fill, int pair, int
  * Process-wide; overrides the environment variable PRISM_B200_GEMM_FILL.  For tests and measurements. */
 int prism_b200_gemm_bf16_fill_mode(int mode);
 
+/* ---- experts: routing, grouped products, products with 4-bit weights --------- */
+
+/*
+ * No counterpart in the reference (its GEMMs are dense: evals/4090_sgemm/runner.cu:245-267,
+ * evals/h100_bench/utils.cuh:504-533).  A token's logits choose k of E experts; the chosen rows are brought into
+ * expert order, multiplied by their expert's matrix, and added up per token.  Sizes that depend on the choice stay on
+ * the device: the products read the group borders (`offsets`) there, and nothing is copied to the host.
+ *
+ * Row matrices are given by a pointer, a width and a row stride `ld` in elements (ld >= width); rows are contiguous
+ * inside.  Outputs must not overlap inputs.  Every call is one launch (route_topk: two above 128 tokens), results
+ * repeat bit for bit, and calls on several streams at once need only outputs (and workspaces) of their own.
+ */
+
+/* Element types of the entry points that take one. */
+enum { PRISM_B200_F32 = 0, PRISM_B200_BF16 = 1, PRISM_B200_F16 = 2 };
+
+/* Bytes of scratch for prism_b200_route_topk (0 up to 128 tokens); 4-byte aligned, its contents do not matter. */
+int prism_b200_route_workspace_size(int tokens, int experts, int k, size_t* bytes);
+
+/*
+ * Chooses, per token, the k experts of the largest logits (tokens x experts, any of the three types) and orders the
+ * chosen rows by expert.
+ *   ids      [tokens][k]   chosen experts, largest logit first, the lowest expert first among equal logits; a logit
+ *                          of -inf or NaN is never chosen: -1 where a token has fewer than k others
+ *   weights  [tokens][k]   softmax over the chosen (renormalize != 0) or over all of the token's logits, in fp32; 0
+ *                          where the id is -1
+ *   offsets  [experts + 1] rows of expert e are offsets[e] .. offsets[e + 1] - 1
+ *   pos      [tokens][k]   row of each choice: by expert, within an expert by token; -1 where the id is -1
+ *   order    [tokens * k]  the choice (token * k + j) of each row; -1 behind the last row
+ * 1 <= experts <= 1024, 1 <= k <= min(experts, 32), tokens * k <= 2^30.  workspace may be NULL where its size is 0.
+ */
+int prism_b200_route_topk(int tokens, int experts, int k, int dtype, const void* logits, long long ld, int renormalize,
+                          int* ids, float* weights, int* pos, int* order, int* offsets, void* workspace, void* stream);
+
+/*
+ * dlogits (tokens x experts, contiguous, the logits' type) from dweights, with the logits, ids and weights of
+ * prism_b200_route_topk (a token's ids are distinct; -1 is passed over).  With renormalize the logits are not read.
+ */
+int prism_b200_route_topk_grad(int tokens, int experts, int k, int dtype, const void* logits, long long ld, int renormalize,
+                               const int* ids, const float* weights, const float* dweights, void* dlogits, void* stream);
+
+/*
+ * out[pos[t][j]] = x[t] (`rows` rows of out exist; a position outside them is passed over, other rows stay as they
+ * are).  Its gradient is prism_b200_route_combine without weights.
+ */
+int prism_b200_route_gather(int dtype, int tokens, int k, int width, const void* x, long long ldx, const int* pos, long long rows,
+                            void* out, long long ldo, void* stream);
+
+/* out[t] = sum over j of weights[t][j] * y[pos[t][j]] in fp32, rounded once; weights may be NULL (all 1). */
+int prism_b200_route_combine(int dtype, int tokens, int k, int width, const void* y, long long ldy, long long rows, const int* pos,
+                             const float* weights, void* out, long long ldo, void* stream);
+
+/*
+ * Gradient of prism_b200_route_combine: dy[pos[t][j]] = weights[t][j] * dout[t] (other rows of dy stay as they are),
+ * dweights[t][j] = dot(dout[t], y[pos[t][j]]) (0 where there is no row).  The positions are distinct.
+ */
+int prism_b200_route_combine_grad(int dtype, int tokens, int k, int width, const void* dout, long long ldd, const void* y,
+                                  long long ldy, long long rows, const int* pos, const float* weights, void* dy, long long lddy,
+                                  float* dweights, void* stream);
+
+/*
+ * Grouped bf16 products on the tensor cores, fp32 accumulation; w is [experts][n][k] contiguous, offsets [experts + 1]
+ * on the device (clamped to 0 .. rows and to non-decreasing borders; rows outside every group are not written).
+ *   prism_b200_grouped_gemm_bf16         out[r] = w[e] x[r]                     x rows x k,  out rows x n
+ *   prism_b200_grouped_gemm_bf16_dgrad   dx[r]  = w[e]^T dy[r]                  dy rows x n, dx rows x k
+ *   prism_b200_grouped_gemm_bf16_wgrad   dw[e]  = sum of dy[r] x[r]^T over e's rows, fp32 or bf16 (out_dtype), zeros for
+ *                                        an empty group; what the rows behind the last group hold does not matter
+ * n and k multiples of 8 (of any size: tiles are cut at the edges), row strides too; pointers 16-byte aligned;
+ * experts <= 1024, rows <= 2^30.
+ */
+int prism_b200_grouped_gemm_bf16(int experts, int rows, int n, int k, const uint16_t* x, long long ldx, const uint16_t* w,
+                                 const int* offsets, uint16_t* out, long long ldo, void* stream);
+int prism_b200_grouped_gemm_bf16_dgrad(int experts, int rows, int n, int k, const uint16_t* dy, long long lddy, const uint16_t* w,
+                                       const int* offsets, uint16_t* dx, long long lddx, void* stream);
+int prism_b200_grouped_gemm_bf16_wgrad(int experts, int rows, int n, int k, const uint16_t* dy, long long lddy, const uint16_t* x,
+                                       long long ldx, const int* offsets, int out_dtype, void* dw, void* stream);
+
+/*
+ * out[r][i] = sum over j of scales[i][j / group] * (q[i][j] - zeros[i][j / group]) * x[r][j], for a few rows r (the weights
+ * are read once for every 8 rows): x, scales and out bf16 or fp16 (dtype), sums in fp32.
+ *   q       [experts][n][k / 2]      two weights of 0 .. 15 per byte, the lower j in the low half
+ *   scales  [experts][n][k / group]
+ *   zeros   [experts][n][k / group]  one byte each, or NULL: 8 everywhere
+ *   offsets [experts + 1]            the rows of each expert's matrix, as above; NULL: one matrix (experts = 1) for all rows
+ * group 32, 64 or 128, k a multiple of it; any n.  x and q 16-byte aligned, ldx a multiple of 8.  A row of x that holds
+ * an infinity or NaN gives outputs that are not finite (possibly NaN where the sum would be an infinity).
+ */
+int prism_b200_gemv_w4(int dtype, int rows, int experts, int n, int k, int group, const void* x, long long ldx, const uint8_t* q,
+                       const void* scales, const uint8_t* zeros, const int* offsets, void* out, long long ldo, void* stream);
+
 /* ---- one-sided all-gather over peer memory --------------------------------- */
 
 /*

@@ -9,7 +9,8 @@ the same order and work in place on device memory:
     runmyh100(M, N, K, A, B, C)                                evals/h100_bench/utils.cuh:504-533
 
 `sgemm`, `scan_` and `gemm_bf16` are thin conveniences over them that read the
-sizes from the tensors.  Everything runs on the current CUDA stream of the
+sizes from the tensors.  `experts` adds the operators of a mixture-of-experts layer
+(route_topk, grouped_gemm_bf16, gemv_w4 and what goes with them).  Everything runs on the current CUDA stream of the
 tensors' device through the C ABI in include/prism_b200.h; there is no CPU or
 PyTorch fallback, and a missing library or a non-zero status raises.
 """
@@ -303,3 +304,9 @@ def gemm_bf16(A: torch.Tensor, B: torch.Tensor, out: torch.Tensor | None = None,
         out = torch.empty((N, M), dtype=torch.bfloat16, device=A.device)
     runmyh100(M, N, K, A, B, out)
     return out
+
+
+from .experts import *  # noqa: E402,F401,F403 -- routing, grouped products, 4-bit weights
+from .experts import __all__ as _experts  # noqa: E402
+
+__all__ += _experts

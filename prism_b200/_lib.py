@@ -6,7 +6,7 @@ call returns a non-zero status, an exception is raised.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_size_t, c_ulonglong, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_ulonglong, c_void_p, POINTER
 from pathlib import Path
 
 from . import build as _build
@@ -51,6 +51,25 @@ SIGNATURES = {
     "prism_b200_scan_static": (c_int, [c_size_t, c_void_p, c_void_p]),
     "prism_b200_gemm_bf16": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
     "prism_b200_gemm_bf16_axpby": (c_int, [c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p]),
+    "prism_b200_route_workspace_size": (c_int, [c_int, c_int, c_int, POINTER(c_size_t)]),
+    "prism_b200_route_topk": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p, c_void_p]),
+    "prism_b200_route_topk_grad": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
+                                           c_void_p]),
+    "prism_b200_route_gather": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong,
+                                        c_void_p]),
+    "prism_b200_route_combine": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p,
+                                         c_longlong, c_void_p]),
+    "prism_b200_route_combine_grad": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_longlong, c_void_p,
+                                              c_void_p, c_void_p, c_longlong, c_void_p, c_void_p]),
+    "prism_b200_grouped_gemm_bf16": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_longlong,
+                                             c_void_p]),
+    "prism_b200_grouped_gemm_bf16_dgrad": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p,
+                                                   c_longlong, c_void_p]),
+    "prism_b200_grouped_gemm_bf16_wgrad": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_int,
+                                                   c_void_p, c_void_p]),
+    "prism_b200_gemv_w4": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_longlong, c_void_p]),
     "prism_b200_peer_push": (c_int, [c_void_p, c_size_t, c_void_p, c_size_t, c_int, c_int, c_void_p, c_int, ctypes.c_uint32, c_void_p, c_void_p]),
     "prism_b200_peer_wait": (c_int, [c_void_p, c_int, c_int, ctypes.c_uint32, c_ulonglong, c_void_p]),
     "prism_b200_host_gemm_bf16_create": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_void_p)]),

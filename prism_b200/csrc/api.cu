@@ -95,6 +95,7 @@ extern "C" int prism_b200_last_error(int* code, char* msg, size_t len) {
             const char* which = st == DEV_SCAN_LOOKBACK_TIMEOUT ? "scan look-back"
                               : st == DEV_SGEMM_PIPE_TIMEOUT    ? "sgemm smem pipeline"
                               : st == DEV_GEMM_PIPE_TIMEOUT     ? "bf16 gemm pipeline"
+                              : st == DEV_GROUPED_PIPE_TIMEOUT  ? "grouped gemm pipeline"
                               : st == DEV_SELFTEST_TIMEOUT      ? "self-test (as requested)"
                               : st == DEV_PEER_WAIT_TIMEOUT     ? "wait for the peers' blocks"
                                                                  : "unknown";

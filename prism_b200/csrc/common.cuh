@@ -29,6 +29,7 @@ enum : uint32_t {
     DEV_SCAN_LOOKBACK_TIMEOUT = 0x5CA10001u,
     DEV_SGEMM_PIPE_TIMEOUT    = 0x56E30001u,  // reserved: the SGEMM kernels have no waits that can run out
     DEV_GEMM_PIPE_TIMEOUT     = 0xB16E0001u,
+    DEV_GROUPED_PIPE_TIMEOUT  = 0xB16E0002u,
     DEV_SELFTEST_TIMEOUT      = 0x5E1F0001u,
     DEV_PEER_WAIT_TIMEOUT     = 0x9EE20001u,
 };
@@ -38,6 +39,24 @@ enum : uint32_t {
         cudaError_t _e = (expr);                                        \
         if (_e != cudaSuccess) return ::prism_b200::cuda_failed(_e, #expr); \
     } while (0)
+
+// ---- argument checks --------------------------------------------------------
+// Whether two row matrices share an element's bytes (both as byte ranges; matrices that interleave by columns of one
+// buffer with one stride do not).
+inline bool rows_overlap(const void* a, long long rows_a, long long width_a, long long ld_a, const void* b, long long rows_b, long long width_b,
+                         long long ld_b, int size) {
+    if (rows_a <= 0 || rows_b <= 0 || width_a <= 0 || width_b <= 0) return false;
+    const unsigned long long a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    const unsigned long long a1 = a0 + ((rows_a - 1) * ld_a + width_a) * size, b1 = b0 + ((rows_b - 1) * ld_b + width_b) * size;
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (ld_a == ld_b) {   // columns of one buffer
+        const unsigned long long pitch = static_cast<unsigned long long>(ld_a) * size;
+        const unsigned long long shift = b0 >= a0 ? (b0 - a0) % pitch : (pitch - (a0 - b0) % pitch) % pitch;
+        if (shift >= static_cast<unsigned long long>(width_a) * size && shift + static_cast<unsigned long long>(width_b) * size <= pitch)
+            return false;
+    }
+    return true;
+}
 
 // ---- device helpers -----------------------------------------------------------
 #ifdef __CUDACC__

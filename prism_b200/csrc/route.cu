@@ -1,0 +1,702 @@
+// Routing of rows to experts: the choice of k experts for each token and the order of the rows that it makes
+// (prism_b200_route_topk), its gradient, and the copies between token order and expert order (gather, combine and
+// combine's gradient).  The grouped products (grouped_gemm.cu, gemv_w4.cu) work on rows in this order.
+//
+// Expert order: row r of expert e lies in [offsets[e], offsets[e + 1]), and within an expert the rows follow their
+// tokens' order, so nothing depends on which block or warp came first.  No kernel here waits for another block: the
+// order is made in two launches (counts per block, then positions) and nothing is added up by floating-point atomics.
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace prism_b200 {
+namespace {
+
+namespace rt {
+constexpr int MAX_EXPERTS = 1024;
+constexpr int MAX_CHOICES = 32;    // lane j of a token's warp holds its choice j
+constexpr int CHUNK = 128;         // tokens whose choices a block ranks at a time
+constexpr int WORDS = CHUNK / 32;
+constexpr int MAX_BLOCKS = 148;    // one block of 32 warps per SM
+constexpr unsigned FULL = 0xffffffffu;
+}  // namespace rt
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// Unsigned integers in the order of the floats.  0 stands for "not to be chosen": -inf, NaN, or no such expert.
+// The two zeros compare equal as floats and so get one key.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    if (!(v > -INFINITY)) return 0u;
+    const uint32_t b = v == 0.f ? 0u : __float_as_uint(v);
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(rt::FULL, v, d);
+    return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(rt::FULL, v, d));
+    return v;
+}
+
+struct RouteArgs {
+    const void* logits;
+    long long ld;
+    int tokens, experts, k, renorm, tokens_per_block;
+    int* ids;
+    float* weights;
+    int* pos;
+    int* order;
+    int* offsets;
+    int* counts;   // [blocks][experts], only with more than one block
+};
+
+// Exclusive prefix sums of EPL * 32 counts by one warp: base[e] = first + sum of count[e'], e' < e; returns the total.
+template <int EPL>
+__device__ __forceinline__ int warp_exclusive_scan(const int* count, int* base, int lane) {
+    int v[EPL], carry = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) v[i] = count[i * 32 + lane];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+        int incl = v[i];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(rt::FULL, incl, d);
+            if (lane >= d) incl += up;
+        }
+        base[i * 32 + lane] = carry + incl - v[i];
+        carry += __shfl_sync(rt::FULL, incl, 31);
+    }
+    return carry;
+}
+
+// One warp per token.  Lane l holds the keys of experts l, l + 32, ...; a round takes the largest key by one
+// redux.sync and the lowest expert that has it by another, so equal logits go to the lowest expert.  Then the block
+// ranks its choices: a token chooses an expert at most once, so a bit per (expert, token) says everything, and the rank
+// of a choice is a popcount of the bits of earlier tokens.  With one block (grid 1, tokens <= CHUNK) the order is
+// complete here; otherwise the ranks are relative to the block and route_place_kernel adds the rest.
+template <typename T, int EPL>
+__global__ void __launch_bounds__(1024, 1) route_choose_kernel(RouteArgs a) {
+    using namespace rt;
+    __shared__ uint32_t mask[EPL * 32][WORDS];
+    __shared__ int running[EPL * 32], base[EPL * 32];
+    __shared__ int16_t chosen[CHUNK * MAX_CHOICES];
+    __shared__ int total;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int k = a.k;
+    const bool single = gridDim.x == 1;
+    const int first = blockIdx.x * a.tokens_per_block;
+    const int last = min(a.tokens, first + a.tokens_per_block);
+    for (int e = threadIdx.x; e < EPL * 32; e += blockDim.x) {
+        running[e] = 0;
+#pragma unroll
+        for (int w = 0; w < WORDS; ++w) mask[e][w] = 0;
+    }
+    __syncthreads();
+    for (int c0 = first; c0 < last; c0 += CHUNK) {
+        const int n = min(CHUNK, last - c0);
+        for (int tt = warp; tt < n; tt += warps) {
+            const size_t t = static_cast<size_t>(c0) + tt;
+            const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+            uint32_t key[EPL];
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) {
+                const int e = i * 32 + lane;
+                key[i] = e < a.experts ? order_key(to_f32(row[e])) : 0u;
+            }
+            uint32_t best = 0;
+            int best_i = 0;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i)
+                if (key[i] > best) best = key[i], best_i = i;
+            uint32_t top = __reduce_max_sync(FULL, best);
+            const float largest = top ? key_value(top) : 0.f;
+            float sum = 0.f;
+            if (!a.renorm) {
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) sum += key[i] ? expf(key_value(key[i]) - largest) : 0.f;
+            }
+            int id = -1;
+            float mine = 0.f;
+            for (int j = 0; j < k && top; ++j) {
+                const int win = __reduce_min_sync(FULL, best == top ? best_i * 32 + lane : 0x7fffffff);
+                if (lane == j) id = win, mine = expf(key_value(top) - largest);
+                if ((win & 31) == lane) {
+                    best = 0;
+#pragma unroll
+                    for (int i = 0; i < EPL; ++i) {
+                        if (i == best_i) key[i] = 0;
+                    }
+#pragma unroll
+                    for (int i = EPL - 1; i >= 0; --i)
+                        if (key[i] >= best && key[i]) best = key[i], best_i = i;
+                }
+                if (j + 1 < k) top = __reduce_max_sync(FULL, best);
+            }
+            sum = warp_sum(a.renorm ? mine : sum);
+            if (lane < k) {
+                a.ids[t * k + lane] = id;
+                a.weights[t * k + lane] = id >= 0 ? mine / sum : 0.f;
+                chosen[tt * MAX_CHOICES + lane] = static_cast<int16_t>(id);
+                if (id >= 0) atomicOr(&mask[id][tt >> 5], 1u << (tt & 31));
+            }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < EPL * 32; e += blockDim.x) {
+            int c = 0;
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) c += __popc(mask[e][w]);
+            base[e] = running[e];
+            running[e] += c;
+        }
+        __syncthreads();
+        if (single) {
+            if (warp == 0) {
+                const int sum = warp_exclusive_scan<EPL>(running, base, lane);
+                for (int e = lane; e < a.experts; e += 32) a.offsets[e] = base[e];
+                if (lane == 0) total = a.offsets[a.experts] = sum;
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < n * k; i += blockDim.x) {
+            const int tt = i / k, j = i - tt * k;
+            const int id = chosen[tt * MAX_CHOICES + j];
+            int p = -1;
+            if (id >= 0) {
+                p = base[id] + __popc(mask[id][tt >> 5] & ((1u << (tt & 31)) - 1u));
+                for (int w = 0; w < (tt >> 5); ++w) p += __popc(mask[id][w]);
+            }
+            const size_t at = static_cast<size_t>(c0) * k + i;
+            a.pos[at] = p;
+            if (single) {
+                if (id >= 0) a.order[p] = static_cast<int>(at);
+                if (static_cast<int>(at) >= total) a.order[at] = -1;
+            }
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < EPL * 32; e += blockDim.x) {
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) mask[e][w] = 0;
+        }
+        __syncthreads();
+    }
+    if (!single)
+        for (int e = threadIdx.x; e < a.experts; e += blockDim.x)
+            a.counts[static_cast<size_t>(blockIdx.x) * a.experts + e] = running[e];
+}
+
+// Second launch with the first one's grid: every block adds up the counts of all blocks (offsets) and of the blocks
+// before it (where its own rows begin), then turns its ranks into positions.  The counts are read once per block from
+// L2 (148 x experts x 4 bytes), which costs less than a third launch.
+template <int EPL>
+__global__ void __launch_bounds__(1024, 1) route_place_kernel(RouteArgs a) {
+    constexpr int EP = EPL * 32;
+    __shared__ int all[EP], before[EP], base[EP];
+    __shared__ int total;
+    const int lane = threadIdx.x & 31;
+    for (int e = threadIdx.x; e < EP; e += blockDim.x) all[e] = before[e] = 0;
+    __syncthreads();
+    {
+        const int e = threadIdx.x % EP, groups = blockDim.x / EP, blocks = gridDim.x;
+        if (e < a.experts) {
+            int sum = 0, pre = 0;
+#pragma unroll 8
+            for (int b = threadIdx.x / EP; b < blocks; b += groups) {
+                const int v = a.counts[static_cast<size_t>(b) * a.experts + e];
+                sum += v;
+                pre += b < static_cast<int>(blockIdx.x) ? v : 0;
+            }
+            atomicAdd(&all[e], sum);
+            atomicAdd(&before[e], pre);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int sum = warp_exclusive_scan<EPL>(all, base, lane);
+        if (blockIdx.x == 0) {
+            for (int e = lane; e < a.experts; e += 32) a.offsets[e] = base[e];
+            if (lane == 0) a.offsets[a.experts] = sum;
+        }
+        if (lane == 0) total = sum;
+    }
+    __syncthreads();
+    const int first = blockIdx.x * a.tokens_per_block;
+    const int last = min(a.tokens, first + a.tokens_per_block);
+    const int end = last * a.k;
+    for (int i = first * a.k + threadIdx.x; i < end; i += blockDim.x) {
+        const int id = a.ids[i];
+        if (id >= 0) {
+            const int p = base[id] + before[id] + a.pos[i];
+            a.pos[i] = p;
+            a.order[p] = i;
+        }
+        if (i >= total) a.order[i] = -1;
+    }
+}
+
+// dl = p * (g - mean) with mean = sum of g * w over the chosen.  renorm: p is w on the chosen and 0 elsewhere, and the
+// logits are not read.  Otherwise p is the softmax over all logits, computed again here (its sum was not kept).
+// One warp per token; the row is first written as if nothing was chosen, then the chosen places are written over.
+template <typename T, int EPL>
+__global__ void __launch_bounds__(256) route_grad_kernel(const T* logits, long long ld, int tokens, int experts, int k,
+                                                         int renorm, const int* ids, const float* weights,
+                                                         const float* dweights, T* out) {
+    const int lane = threadIdx.x & 31;
+    const size_t t = static_cast<size_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (t >= static_cast<size_t>(tokens)) return;
+    int id = -1;
+    float w = 0.f, g = 0.f;
+    if (lane < k) {
+        id = ids[t * k + lane];
+        if (id >= experts) id = -1;
+        if (id >= 0) w = weights[t * k + lane], g = dweights[t * k + lane];
+    }
+    const float mean = warp_sum(id >= 0 ? g * w : 0.f);
+    T* row = out + t * experts;
+    float p = w;
+    if (renorm) {
+        for (int e = lane; e < experts; e += 32) row[e] = from_f32<T>(0.f);
+    } else {
+        const T* in = logits + t * ld;
+        float v[EPL];
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            const int e = i * 32 + lane;
+            v[i] = e < experts ? to_f32(in[e]) : -INFINITY;
+            top = fmaxf(top, v[i]);   // a NaN (never chosen) does not enter
+        }
+        top = warp_max(top);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) sum += v[i] > -INFINITY ? expf(v[i] - top) : 0.f;
+        sum = warp_sum(sum);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            const int e = i * 32 + lane;
+            if (e < experts) row[e] = from_f32<T>(v[i] > -INFINITY ? expf(v[i] - top) / sum * -mean : 0.f);
+        }
+        p = id >= 0 ? expf(to_f32(in[id]) - top) / sum : 0.f;
+    }
+    __syncwarp();
+    if (id >= 0) row[id] = from_f32<T>(p * (g - mean));
+}
+
+// ---- copies between token order and expert order --------------------------------------------------------------
+// Memory-bound: every source row is read once and every destination row written once.  threadIdx.x walks a row in
+// vectors, threadIdx.y the tokens of a block, blockIdx.y the pieces of a long row.
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+    T v[V];
+};
+
+// out[pos[t, j]] = x[t]; U: raw unit of the copy.
+template <typename U>
+__global__ void __launch_bounds__(256) route_gather_kernel(const U* x, long long ldx, int tokens, int k, int units, const int* pos,
+                                                           long long rows, U* out, long long ldo) {
+    const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (t >= static_cast<size_t>(tokens)) return;
+    const U* src = x + t * ldx;
+    const int* p = pos + t * k;
+    for (int c = blockIdx.y * blockDim.x * 2 + threadIdx.x; c < units; c += gridDim.y * blockDim.x * 2) {
+        const int c2 = c + blockDim.x;
+        const U v = src[c];
+        const U v2 = c2 < units ? src[c2] : v;
+        for (int j = 0; j < k; ++j) {
+            const int r = p[j];
+            if (r < 0 || r >= rows) continue;
+            U* dst = out + static_cast<size_t>(r) * ldo;
+            dst[c] = v;
+            if (c2 < units) dst[c2] = v2;
+        }
+    }
+}
+
+// out[t] = sum over j of w[t, j] * y[pos[t, j]], added up in fp32 in the order of j and rounded once.
+template <typename T, int V>
+__global__ void __launch_bounds__(256) route_combine_kernel(const T* y, long long ldy, long long rows, int tokens, int k, int units,
+                                                            const int* pos, const float* weights, T* out, long long ldo) {
+    using W = Vec<T, V>;
+    const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (t >= static_cast<size_t>(tokens)) return;
+    const int* p = pos + t * k;
+    const float* wt = weights ? weights + t * k : nullptr;
+    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < units; c += gridDim.y * blockDim.x) {
+        float acc[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        for (int j0 = 0; j0 < k; j0 += 4) {   // four rows in flight
+            W v[4];
+            bool live[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int r = j0 + u < k ? p[j0 + u] : -1;
+                live[u] = r >= 0 && r < rows;
+                if (live[u]) v[u] = *reinterpret_cast<const W*>(y + static_cast<size_t>(r) * ldy + static_cast<size_t>(c) * V);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (!live[u]) continue;
+                const float w = wt ? wt[j0 + u] : 1.f;
+#pragma unroll
+                for (int i = 0; i < V; ++i) acc[i] = fmaf(w, to_f32(v[u].v[i]), acc[i]);
+            }
+        }
+        W o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(acc[i]);
+        *reinterpret_cast<W*>(out + t * ldo + static_cast<size_t>(c) * V) = o;
+    }
+}
+
+// dy[pos[t, j]] = w[t, j] * dout[t] and dw[t, j] = dot(dout[t], y[pos[t, j]]): one pass over the rows, the dot products
+// in fp32 in registers (KT of them), added up over the token's threads by shuffles and then in warp order.
+template <typename T, int V, int KT>
+__global__ void __launch_bounds__(256) route_combine_grad_kernel(const T* dout, long long ldd, const T* y, long long ldy,
+                                                                 long long rows, int tokens, int k, int units, const int* pos,
+                                                                 const float* weights, T* dy, long long lddy, float* dw) {
+    using W = Vec<T, V>;
+    __shared__ float part[8][KT];
+    const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const bool here = t < static_cast<size_t>(tokens);   // blockDim.x is a multiple of 32: whole warps
+    const int warps_x = blockDim.x >> 5, warp_x = threadIdx.x >> 5;
+    float acc[KT];
+#pragma unroll
+    for (int j = 0; j < KT; ++j) acc[j] = 0.f;
+    if (here) {
+        const int* p = pos + t * k;
+        int r[KT];
+        float w[KT];
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+            r[j] = j < k ? p[j] : -1;
+            if (r[j] >= rows) r[j] = -1;
+            w[j] = r[j] >= 0 ? weights[t * k + j] : 0.f;
+        }
+        for (int c = threadIdx.x; c < units; c += blockDim.x) {
+            const W d = *reinterpret_cast<const W*>(dout + t * ldd + static_cast<size_t>(c) * V);
+            float df[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) df[i] = to_f32(d.v[i]);
+#pragma unroll
+            for (int j = 0; j < KT; ++j) {
+                if (r[j] < 0) continue;
+                const W a = *reinterpret_cast<const W*>(y + static_cast<size_t>(r[j]) * ldy + static_cast<size_t>(c) * V);
+                W o;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    acc[j] = fmaf(df[i], to_f32(a.v[i]), acc[j]);
+                    o.v[i] = from_f32<T>(w[j] * df[i]);
+                }
+                *reinterpret_cast<W*>(dy + static_cast<size_t>(r[j]) * lddy + static_cast<size_t>(c) * V) = o;
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < KT; ++j) acc[j] = warp_sum(acc[j]);
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+        for (int j = 0; j < KT; ++j) part[threadIdx.y * warps_x + warp_x][j] = acc[j];
+    }
+    __syncthreads();
+    if (here && threadIdx.x < static_cast<unsigned>(k)) {
+        float s = 0.f;
+        for (int i = 0; i < warps_x; ++i) s += part[threadIdx.y * warps_x + i][threadIdx.x];
+        dw[t * k + threadIdx.x] = s;
+    }
+}
+
+int blocks_for(int tokens) {
+    if (tokens <= rt::CHUNK) return 1;
+    const int by_warp = (tokens + 31) / 32;   // a token per warp while that leaves SMs without a block
+    return by_warp < rt::MAX_BLOCKS ? by_warp : rt::MAX_BLOCKS;
+}
+
+int check_choice(const char* fn, int tokens, int experts, int k) {
+    if (tokens < 0 || experts < 0 || k < 0) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+    if (experts < 1 || experts > rt::MAX_EXPERTS)
+        return set_error(PRISM_B200_ERR_UNSUPPORTED_SHAPE, "%s: 1 to %d experts (got %d)", fn, rt::MAX_EXPERTS, experts);
+    if (k < 1 || k > experts || k > rt::MAX_CHOICES)
+        return set_error(PRISM_B200_ERR_UNSUPPORTED_SHAPE, "%s: 1 to min(experts, %d) choices (got %d)", fn, rt::MAX_CHOICES, k);
+    if (static_cast<long long>(tokens) * k > 1LL << 30)
+        return set_error(PRISM_B200_ERR_TOO_LARGE, "%s: tokens x k at most 2^30", fn);
+    return PRISM_B200_OK;
+}
+
+int check_rows(const char* fn, long long ld, long long width) {
+    if (ld < width) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "%s: a row stride below the row's width", fn);
+    return PRISM_B200_OK;
+}
+
+int elem_size(int dtype) { return dtype == PRISM_B200_F32 ? 4 : (dtype == PRISM_B200_BF16 || dtype == PRISM_B200_F16) ? 2 : 0; }
+
+// Largest vector, in elements, that divides the width, the strides and the addresses (at most 16 bytes).
+int vector_elems(int size, long long width, long long ld_a, const void* a, long long ld_b, const void* b, long long ld_c = 0,
+                 const void* c = nullptr) {
+    int v = 16 / size;
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c);
+    while (v > 1 && (width % v || ld_a % v || ld_b % v || ld_c % v || addr % (static_cast<uintptr_t>(v) * size))) v >>= 1;
+    return v;
+}
+
+template <typename T>
+int launch_choose(const RouteArgs& a, int blocks, int threads, cudaStream_t s) {
+    const int per_lane = (a.experts + 31) / 32;
+    if (per_lane <= 1) route_choose_kernel<T, 1><<<blocks, threads, 0, s>>>(a);
+    else if (per_lane <= 2) route_choose_kernel<T, 2><<<blocks, threads, 0, s>>>(a);
+    else if (per_lane <= 4) route_choose_kernel<T, 4><<<blocks, threads, 0, s>>>(a);
+    else if (per_lane <= 8) route_choose_kernel<T, 8><<<blocks, threads, 0, s>>>(a);
+    else if (per_lane <= 16) route_choose_kernel<T, 16><<<blocks, threads, 0, s>>>(a);
+    else route_choose_kernel<T, 32><<<blocks, threads, 0, s>>>(a);
+    PRISM_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    return PRISM_B200_OK;
+}
+
+int launch_place(const RouteArgs& a, int blocks, cudaStream_t s) {
+    const int per_lane = (a.experts + 31) / 32;
+    if (per_lane <= 1) route_place_kernel<1><<<blocks, 1024, 0, s>>>(a);
+    else if (per_lane <= 2) route_place_kernel<2><<<blocks, 1024, 0, s>>>(a);
+    else if (per_lane <= 4) route_place_kernel<4><<<blocks, 1024, 0, s>>>(a);
+    else if (per_lane <= 8) route_place_kernel<8><<<blocks, 1024, 0, s>>>(a);
+    else if (per_lane <= 16) route_place_kernel<16><<<blocks, 1024, 0, s>>>(a);
+    else route_place_kernel<32><<<blocks, 1024, 0, s>>>(a);
+    PRISM_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    return PRISM_B200_OK;
+}
+
+template <typename T>
+int launch_grad(const void* logits, long long ld, int tokens, int experts, int k, int renorm, const int* ids, const float* weights,
+                const float* dweights, void* out, cudaStream_t s) {
+    const int blocks = (tokens + 7) / 8;
+    const int per_lane = (experts + 31) / 32;
+    const T* l = static_cast<const T*>(logits);
+    T* o = static_cast<T*>(out);
+    if (renorm || per_lane <= 1) route_grad_kernel<T, 1><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
+    else if (per_lane <= 4) route_grad_kernel<T, 4><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
+    else if (per_lane <= 8) route_grad_kernel<T, 8><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
+    else route_grad_kernel<T, 32><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
+    PRISM_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    return PRISM_B200_OK;
+}
+
+// Threads along a row (a power of two, at least `least`) and tokens per block of 256 threads.
+dim3 row_block(int units, int least) {
+    int x = least;
+    while (x < 256 && x < units) x <<= 1;
+    return dim3(static_cast<unsigned>(x), static_cast<unsigned>(256 / x));
+}
+
+template <typename U>
+int launch_gather(const void* x, long long ldx, int tokens, int k, int units, const int* pos, long long rows, void* out, long long ldo,
+                  cudaStream_t s) {
+    const dim3 block = row_block(units, 16);
+    const int pieces = (units + 511) / 512;
+    const dim3 grid((tokens + block.y - 1) / block.y, pieces < 64 ? pieces : 64);
+    route_gather_kernel<U><<<grid, block, 0, s>>>(static_cast<const U*>(x), ldx, tokens, k, units, pos, rows, static_cast<U*>(out), ldo);
+    PRISM_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    return PRISM_B200_OK;
+}
+
+template <typename T, int V>
+int launch_combine(const void* y, long long ldy, long long rows, int tokens, int k, int width, const int* pos, const float* weights,
+                   void* out, long long ldo, cudaStream_t s) {
+    const int units = width / V;
+    const dim3 block = row_block(units, 16);
+    const int pieces = (units + 255) / 256;
+    const dim3 grid((tokens + block.y - 1) / block.y, pieces < 64 ? pieces : 64);
+    route_combine_kernel<T, V><<<grid, block, 0, s>>>(static_cast<const T*>(y), ldy, rows, tokens, k, units, pos, weights,
+                                                      static_cast<T*>(out), ldo);
+    PRISM_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    return PRISM_B200_OK;
+}
+
+struct CombineGrad {
+    const void *dout, *y;
+    void* dy;
+    long long ldd, ldy, lddy, rows;
+    int tokens, k, width;
+    const int* pos;
+    const float* weights;
+    float* dw;
+};
+
+template <typename T, int V, int KT>
+int launch_combine_grad_k(const CombineGrad& a, cudaStream_t s) {
+    const int units = a.width / V;
+    const dim3 block = row_block(units, 32);
+    const unsigned grid = (a.tokens + block.y - 1) / block.y;
+    route_combine_grad_kernel<T, V, KT><<<grid, block, 0, s>>>(static_cast<const T*>(a.dout), a.ldd, static_cast<const T*>(a.y), a.ldy,
+                                                               a.rows, a.tokens, a.k, units, a.pos, a.weights, static_cast<T*>(a.dy),
+                                                               a.lddy, a.dw);
+    PRISM_CUDA_TRY(cudaGetLastError());
+    count_launch();
+    return PRISM_B200_OK;
+}
+
+template <typename T, int V>
+int launch_combine_grad(const CombineGrad& a, cudaStream_t s) {
+    if (a.k <= 2) return launch_combine_grad_k<T, V, 2>(a, s);
+    if (a.k <= 4) return launch_combine_grad_k<T, V, 4>(a, s);
+    if (a.k <= 8) return launch_combine_grad_k<T, V, 8>(a, s);
+    return launch_combine_grad_k<T, V, 32>(a, s);
+}
+
+}  // namespace
+}  // namespace prism_b200
+
+using namespace prism_b200;
+
+extern "C" int prism_b200_route_workspace_size(int tokens, int experts, int k, size_t* bytes) {
+    if (!bytes) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_workspace_size: null pointer");
+    if (int rc = check_choice("route_workspace_size", tokens, experts, k)) return rc;
+    const int blocks = blocks_for(tokens);
+    *bytes = blocks == 1 ? 0 : static_cast<size_t>(blocks) * experts * sizeof(int);
+    return PRISM_B200_OK;
+}
+
+extern "C" int prism_b200_route_topk(int tokens, int experts, int k, int dtype, const void* logits, long long ld, int renormalize,
+                                     int* ids, float* weights, int* pos, int* order, int* offsets, void* workspace, void* stream) {
+    if (int rc = check_choice("route_topk", tokens, experts, k)) return rc;
+    if (!elem_size(dtype)) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_topk: unknown element type %d", dtype);
+    const int blocks = blocks_for(tokens);
+    if (!offsets || (tokens > 0 && (!logits || !ids || !weights || !pos || !order)) || (blocks > 1 && !workspace))
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_topk: null pointer");
+    if (int rc = check_rows("route_topk", ld, experts)) return rc;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tokens == 0) {
+        PRISM_CUDA_TRY(cudaMemsetAsync(offsets, 0, (static_cast<size_t>(experts) + 1) * sizeof(int), s));
+        return PRISM_B200_OK;
+    }
+    RouteArgs a{logits, ld, tokens, experts, k, renormalize ? 1 : 0, (tokens + blocks - 1) / blocks, ids, weights, pos, order, offsets,
+                static_cast<int*>(workspace)};
+    // a warp per token, up to 32 of them; at least four so that the ranking of many experts is not left to one warp
+    int threads = 32 * a.tokens_per_block;
+    threads = threads < 128 ? 128 : threads > 1024 ? 1024 : threads;
+    int rc = dtype == PRISM_B200_F32    ? launch_choose<float>(a, blocks, threads, s)
+             : dtype == PRISM_B200_BF16 ? launch_choose<__nv_bfloat16>(a, blocks, threads, s)
+                                        : launch_choose<__half>(a, blocks, threads, s);
+    if (rc || blocks == 1) return rc;
+    return launch_place(a, blocks, s);
+}
+
+extern "C" int prism_b200_route_topk_grad(int tokens, int experts, int k, int dtype, const void* logits, long long ld, int renormalize,
+                                          const int* ids, const float* weights, const float* dweights, void* dlogits, void* stream) {
+    if (int rc = check_choice("route_topk_grad", tokens, experts, k)) return rc;
+    if (!elem_size(dtype)) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_topk_grad: unknown element type %d", dtype);
+    if (tokens == 0) return PRISM_B200_OK;
+    if (!logits || !ids || !weights || !dweights || !dlogits)
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_topk_grad: null pointer");
+    if (int rc = check_rows("route_topk_grad", ld, experts)) return rc;
+    if (rows_overlap(dlogits, tokens, experts, experts, logits, tokens, experts, ld, elem_size(dtype)))
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_topk_grad: dlogits and logits overlap");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == PRISM_B200_F32) return launch_grad<float>(logits, ld, tokens, experts, k, renormalize, ids, weights, dweights, dlogits, s);
+    if (dtype == PRISM_B200_BF16)
+        return launch_grad<__nv_bfloat16>(logits, ld, tokens, experts, k, renormalize, ids, weights, dweights, dlogits, s);
+    return launch_grad<__half>(logits, ld, tokens, experts, k, renormalize, ids, weights, dweights, dlogits, s);
+}
+
+namespace prism_b200 {
+namespace {
+int check_copy(const char* fn, int dtype, int tokens, int k, int width, long long rows, long long ld_a, long long ld_b) {
+    if (!elem_size(dtype)) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", fn, dtype);
+    if (tokens < 0 || k < 0 || width < 0 || rows < 0) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "%s: negative size", fn);
+    if (k < 1 || k > rt::MAX_CHOICES)
+        return set_error(PRISM_B200_ERR_UNSUPPORTED_SHAPE, "%s: 1 to %d choices (got %d)", fn, rt::MAX_CHOICES, k);
+    if (static_cast<long long>(tokens) * k > 1LL << 30)
+        return set_error(PRISM_B200_ERR_TOO_LARGE, "%s: tokens x k at most 2^30", fn);
+    if (int rc = check_rows(fn, ld_a, width)) return rc;
+    return check_rows(fn, ld_b, width);
+}
+}  // namespace
+}  // namespace prism_b200
+
+extern "C" int prism_b200_route_gather(int dtype, int tokens, int k, int width, const void* x, long long ldx, const int* pos,
+                                       long long rows, void* out, long long ldo, void* stream) {
+    if (int rc = check_copy("route_gather", dtype, tokens, k, width, rows, ldx, ldo)) return rc;
+    if (tokens == 0 || width == 0 || rows == 0) return PRISM_B200_OK;
+    if (!x || !pos || !out) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_gather: null pointer");
+    const int size = elem_size(dtype);
+    if (rows_overlap(x, tokens, width, ldx, out, rows, width, ldo, size))
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_gather: x and out overlap");
+    const int v = vector_elems(size, width, ldx, x, ldo, out), unit = v * size;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (unit == 16) return launch_gather<uint4>(x, ldx / v, tokens, k, width / v, pos, rows, out, ldo / v, s);
+    if (unit == 8) return launch_gather<uint2>(x, ldx / v, tokens, k, width / v, pos, rows, out, ldo / v, s);
+    if (unit == 4) return launch_gather<uint32_t>(x, ldx / v, tokens, k, width / v, pos, rows, out, ldo / v, s);
+    return launch_gather<uint16_t>(x, ldx / v, tokens, k, width / v, pos, rows, out, ldo / v, s);
+}
+
+extern "C" int prism_b200_route_combine(int dtype, int tokens, int k, int width, const void* y, long long ldy, long long rows,
+                                        const int* pos, const float* weights, void* out, long long ldo, void* stream) {
+    if (int rc = check_copy("route_combine", dtype, tokens, k, width, rows, ldy, ldo)) return rc;
+    if (tokens == 0 || width == 0) return PRISM_B200_OK;
+    if ((!y && rows > 0) || !pos || !out) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_combine: null pointer");
+    const int size = elem_size(dtype);
+    if (rows_overlap(y, rows, width, ldy, out, tokens, width, ldo, size))
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_combine: y and out overlap");
+    const int v = vector_elems(size, width, ldy, y, ldo, out);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+#define COMBINE(T, V) return launch_combine<T, V>(y, ldy, rows, tokens, k, width, pos, weights, out, ldo, s)
+    if (dtype == PRISM_B200_F32) {
+        if (v == 4) COMBINE(float, 4);
+        if (v == 2) COMBINE(float, 2);
+        COMBINE(float, 1);
+    }
+    if (dtype == PRISM_B200_BF16) {
+        if (v == 8) COMBINE(__nv_bfloat16, 8);
+        if (v >= 2) COMBINE(__nv_bfloat16, 2);
+        COMBINE(__nv_bfloat16, 1);
+    }
+    if (v == 8) COMBINE(__half, 8);
+    if (v >= 2) COMBINE(__half, 2);
+    COMBINE(__half, 1);
+#undef COMBINE
+}
+
+extern "C" int prism_b200_route_combine_grad(int dtype, int tokens, int k, int width, const void* dout, long long ldd, const void* y,
+                                             long long ldy, long long rows, const int* pos, const float* weights, void* dy,
+                                             long long lddy, float* dweights, void* stream) {
+    if (int rc = check_copy("route_combine_grad", dtype, tokens, k, width, rows, ldd, ldy)) return rc;
+    if (int rc = check_rows("route_combine_grad", lddy, width)) return rc;
+    if (tokens == 0) return PRISM_B200_OK;
+    if (((!y || !dy) && rows > 0 && width > 0) || (!dout && width > 0) || !pos || !weights || !dweights)
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_combine_grad: null pointer");
+    const int size = elem_size(dtype);
+    if (rows_overlap(dy, rows, width, lddy, y, rows, width, ldy, size) || rows_overlap(dy, rows, width, lddy, dout, tokens, width, ldd, size))
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "route_combine_grad: dy overlaps y or dout");
+    const CombineGrad a{dout, y, dy, ldd, ldy, lddy, rows, tokens, k, width, pos, weights, dweights};
+    const int v = vector_elems(size, width, ldd, dout, ldy, y, lddy, dy);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == PRISM_B200_F32) {
+        if (v == 4) return launch_combine_grad<float, 4>(a, s);
+        return v == 2 ? launch_combine_grad<float, 2>(a, s) : launch_combine_grad<float, 1>(a, s);
+    }
+    if (dtype == PRISM_B200_BF16) {
+        if (v == 8) return launch_combine_grad<__nv_bfloat16, 8>(a, s);
+        return v >= 2 ? launch_combine_grad<__nv_bfloat16, 2>(a, s) : launch_combine_grad<__nv_bfloat16, 1>(a, s);
+    }
+    if (v == 8) return launch_combine_grad<__half, 8>(a, s);
+    return v >= 2 ? launch_combine_grad<__half, 2>(a, s) : launch_combine_grad<__half, 1>(a, s);
+}

@@ -1,0 +1,127 @@
+"""The operators of a mixture-of-experts layer as they are used together: forward, backward and the 4-bit form."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+BF = torch.bfloat16
+
+
+def make(T, E, k, H, F, seed=0, masked=0.1):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    randn = lambda *s: torch.randn(s, device=DEV, generator=g)  # noqa: E731
+    logits = randn(T, E)
+    if masked:
+        logits[torch.rand((T,), device=DEV, generator=g) < masked] = float("-inf")
+    return logits, randn(T, H).to(BF), (randn(E, F, H) / H ** 0.5).to(BF), (randn(E, H, F) / F ** 0.5).to(BF), randn(T, H).to(BF)
+
+
+def layer(pb, logits, x, w1, w2, dout, k):
+    """Forward and backward of y = sum of weights * relu(x w1') w2' over the chosen experts."""
+    r = pb.route_topk(logits, k)
+    xs = pb.route_gather(x, r.pos)
+    h = pb.grouped_gemm_bf16(xs, w1, r.offsets)
+    act = torch.relu(h)
+    ys = pb.grouped_gemm_bf16(act, w2, r.offsets)
+    y = pb.route_combine(ys, r.pos, r.weights)
+    dys, dweights = pb.route_combine_grad(dout, ys, r.pos, r.weights)
+    dact = pb.grouped_gemm_bf16_dgrad(dys, w2, r.offsets)
+    dw2 = pb.grouped_gemm_bf16_wgrad(dys, act, r.offsets, dtype=torch.float32)
+    dh = torch.where(h > 0, dact, torch.zeros_like(dact))
+    dxs = pb.grouped_gemm_bf16_dgrad(dh, w1, r.offsets)
+    dw1 = pb.grouped_gemm_bf16_wgrad(dh, xs, r.offsets, dtype=torch.float32)
+    dx = pb.route_combine(dxs, r.pos)
+    dlogits = pb.route_topk_grad(logits, r.ids, r.weights, dweights)
+    return {"y": y, "dx": dx, "dw1": dw1, "dw2": dw2, "dlogits": dlogits}, r
+
+
+def plain(logits, x, w1, w2, dout, ids):
+    """The same in fp64 with autograd, a token at a time over its experts by one-hot sums."""
+    E = w1.shape[0]
+    args = [t.double().requires_grad_() for t in (logits, x, w1, w2)]
+    l, x, w1, w2 = args
+    chosen = torch.zeros(l.shape, dtype=torch.bool, device=DEV)
+    t, j = (ids >= 0).nonzero(as_tuple=True)
+    chosen[t, ids[t, j].long()] = True
+    kept = torch.where(chosen, l, torch.full_like(l, -1e30))
+    gate = torch.where(chosen, torch.softmax(kept, 1), torch.zeros_like(l))
+    y = 0
+    for e in range(E):
+        y = y + gate[:, e:e + 1] * (torch.relu(x @ w1[e].t()) @ w2[e].t())
+    grads = torch.autograd.grad(y, args, dout.double())
+    return {"y": y.detach(), "dlogits": torch.where(chosen, grads[0], 0.0), "dx": grads[1], "dw1": grads[2], "dw2": grads[3]}
+
+
+@pytest.mark.parametrize("T,E,k,H,F", [(1, 4, 2, 64, 128), (50, 8, 2, 128, 192), (700, 16, 4, 256, 320)])
+def test_layer_and_its_gradients(pb, T, E, k, H, F):
+    inputs = make(T, E, k, H, F, seed=T, masked=0.0 if T == 1 else 0.1)
+    got, r = layer(pb, *inputs, k)
+    want = plain(*inputs, r.ids)
+    # Up to four values in a row are rounded to bf16 on the way (h, ys or dys, dact, the output): 2^-8 of each at most,
+    # and the relu's border moves by h's rounding.  Over a whole tensor the roundings are independent and half that on
+    # average, so 4 * 2^-8 bounds the norm of the difference.
+    for name, value in got.items():
+        off = (value.double() - want[name]).norm() / want[name].norm().clamp(min=1e-30)
+        assert off <= 4 * 2.0 ** -8, (name, float(off))
+
+
+def test_captured_layer_with_other_tokens(pb):
+    """Forward and backward in one graph; replayed for tokens that choose other experts."""
+    T, E, k, H, F = 300, 8, 2, 128, 256
+    inputs = make(T, E, k, H, F, seed=1)
+    layer(pb, *inputs, k)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, r = layer(pb, *inputs, k)
+    fresh = make(T, E, k, H, F, seed=2)
+    for a, b in zip(inputs, fresh):
+        a.copy_(b)
+    graph.replay()
+    torch.cuda.synchronize()
+    want, r2 = layer(pb, *fresh, k)
+    assert torch.equal(r.ids, r2.ids) and torch.equal(r.offsets, r2.offsets)
+    for name in got:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_decoding_with_4_bit_experts(pb):
+    """The layer's forward with 4-bit matrices is the one with the matrices they stand for."""
+    T, E, k, H, F, G = 5, 16, 4, 256, 512, 64
+    logits, x, _, _, _ = make(T, E, k, H, F, seed=3, masked=0.0)
+    g = torch.Generator(device=DEV).manual_seed(4)
+
+    def quantised(n, kk):
+        q = torch.randint(0, 256, (E, n, kk // 2), dtype=torch.uint8, device=DEV, generator=g)
+        s = 2.0 ** torch.randint(-7, -4, (E, n, kk // G), device=DEV, generator=g).to(BF)   # scale * (q - 8) is a bf16 number
+        v = torch.stack([q & 15, q >> 4], dim=-1).flatten(-2).float() - 8
+        return q, s, (v * s.float().repeat_interleave(G, -1)).to(BF)
+
+    q1, s1, w1 = quantised(F, H)
+    q2, s2, w2 = quantised(H, F)
+    r = pb.route_topk(logits, k)
+    xs = pb.route_gather(x, r.pos)
+    a = torch.relu(pb.gemv_w4(xs, q1, s1, offsets=r.offsets))
+    b = torch.relu(pb.grouped_gemm_bf16(xs, w1, r.offsets))
+    # the same products added up in fp32 in another order: the bf16 results are equal or neighbours
+    assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-4).all()
+    ya = pb.route_combine(pb.gemv_w4(b, q2, s2, offsets=r.offsets), r.pos, r.weights)
+    yb = pb.route_combine(pb.grouped_gemm_bf16(b, w2, r.offsets), r.pos, r.weights)
+    assert ((ya.float() - yb.float()).abs() <= 3 * 2.0 ** -7 * yb.float().abs().amax()).all()
+
+
+def test_results_repeat(pb):
+    inputs = make(900, 32, 4, 128, 256, seed=7)
+    first, _ = layer(pb, *inputs, 4)
+    for _ in range(3):
+        again, _ = layer(pb, *inputs, 4)
+        assert all(torch.equal(first[n], again[n]) for n in first)
+
+
+def test_wrong_device_is_refused(pb):
+    logits, x, w1, _, _ = make(10, 4, 2, 64, 64)
+    r = pb.route_topk(logits, 2)
+    with pytest.raises(TypeError):
+        pb.route_gather(x.cpu(), r.pos)
+    with pytest.raises(TypeError):
+        pb.grouped_gemm_bf16(x, w1, r.offsets.cpu())
