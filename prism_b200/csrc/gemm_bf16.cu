@@ -354,29 +354,6 @@ struct PairCfg {
 };
 }  // namespace g16
 
-// Unwind path of the two-CTA kernels' producers: loads already issued must land before the CTA gives
-// its shared memory back.  All loads of a pair complete on the LEADER's "full" barriers, so the
-// leader waits for the armed ones (never_flag stays 0, so the wait is not cut short by the abort
-// flag); the other CTA cannot watch those barriers and instead lets the longest a load can take
-// pass.  Both are bounded.
-__device__ __forceinline__ void drain_pair_loads(uint64_t* full_bar, int stage, uint32_t phase, int armed, int stages,
-                                                 bool leader, volatile uint32_t* never_flag) {
-    if (leader) {
-        int s = stage;
-        uint32_t ph = phase;
-        for (int i = 0; i < armed; ++i) {
-            if (--s < 0) {
-                s = stages - 1;
-                ph ^= 1u;
-            }
-            mbar_wait_bounded(&full_bar[s], ph, never_flag, 2000000ull);
-        }
-    } else if (armed > 0) {
-        const unsigned long long t0 = global_timer_ns();
-        while (global_timer_ns() - t0 < 200000ull) __nanosleep(1000);
-    }
-}
-
 template <int GROUP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(g16::THREADS, 1)
 cutlass_my_h100_match_no_tail_pair(int M, int N, int K, __nv_bfloat16* C, const __grid_constant__ CUtensorMap tensorMapA,

@@ -17,6 +17,7 @@ tokens * k rows hold their groups in front; what lies behind offsets[-1] is neit
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -85,18 +86,22 @@ def _code(name: str, dtype) -> int:
 
 def _run(device, fn, *args) -> None:
     """fn(*args, current stream of `device`) with that device current."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = torch._C._cuda_getCurrentRawStream(device.index)   # torch.cuda.current_stream(device).cuda_stream, 2 us sooner
     if device.index == torch.cuda.current_device():
-        _lib.check(fn(*args, stream))
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, stream))
+            status = fn(*args, stream)
+    if status:
+        _lib.check(status)
 
 
 # ---------------------------------------------------------------------------
 # routing
 # ---------------------------------------------------------------------------
+@functools.lru_cache(maxsize=256)
 def route_workspace_size(tokens: int, experts: int, k: int) -> int:
+    """Bytes of scratch that route_topk needs (0 up to 128 tokens)."""
     out = ctypes.c_size_t(0)
     _lib.check(load().prism_b200_route_workspace_size(int(tokens), int(experts), int(k), ctypes.byref(out)))
     return int(out.value)
