@@ -1,6 +1,7 @@
 // Library-level entry points: version, sticky error state, launch counter and
 // the pinned status word that kernels use to report a wait that ran out.
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 #include <atomic>
 #include <cstdarg>
@@ -53,6 +54,31 @@ uint32_t* device_status_word() {
     return g_status;
 }
 
+int encode_tensor_map(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* ptr, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+    using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                       const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                       CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static std::mutex mu;
+    static EncodeTiledFn fn = nullptr;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!fn) {
+            void* p = nullptr;
+            cudaDriverEntryPointQueryResult q;
+            cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+            if (e != cudaSuccess || !p || q != cudaDriverEntryPointSuccess)
+                return set_error(PRISM_B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+        }
+    }
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(out, type, rank, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(PRISM_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
+    return PRISM_B200_OK;
+}
+
 }  // namespace prism_b200
 
 using namespace prism_b200;
@@ -96,6 +122,7 @@ extern "C" int prism_b200_last_error(int* code, char* msg, size_t len) {
                               : st == DEV_SGEMM_PIPE_TIMEOUT    ? "sgemm smem pipeline"
                               : st == DEV_GEMM_PIPE_TIMEOUT     ? "bf16 gemm pipeline"
                               : st == DEV_GROUPED_PIPE_TIMEOUT  ? "grouped gemm pipeline"
+                              : st == DEV_GEMV_PIPE_TIMEOUT     ? "4-bit product pipeline"
                               : st == DEV_SELFTEST_TIMEOUT      ? "self-test (as requested)"
                               : st == DEV_PEER_WAIT_TIMEOUT     ? "wait for the peers' blocks"
                                                                  : "unknown";

@@ -15,10 +15,16 @@
 //     pairs are (k, k + 4) as the masks deliver them, and x is brought into that order by four PRMTs per 8 values.
 //   * The four lanes of a quad take the four words of 32 consecutive k, so a group of 32, 64 or 128 is 1, 2 or 4 steps
 //     and its sum is complete in the accumulator when its scale is applied (fp32).
-//   * A warp owns 32 weight rows and every 8th slice of 128 k; slices (and the rows of x that go with them) arrive by
-//     cp.async in a ring of the warp's own, which runs on across work items: no block barrier is between a load and
-//     its use.  The eight warps' sums meet in shared memory once per item, added in warp order.
+//   * A warp takes 32 weight rows and a share of k in slices of 128; `split` warps share the same rows, so that long rows
+//     are split and short ones are not (four slices per warp where there are enough).  A slice (2 KB of weights, and its
+//     256 bytes of each row of x) is two TMA copies into a ring of the warp's own, issued by one lane; the ring runs on
+//     across work items, so no block barrier is between a copy and its use.  The copies' 64-byte swizzle keeps a step's
+//     reads free of bank conflicts, and what lies outside the matrices arrives as zeros.
+//   * The warps' sums meet in shared memory once per item, added in warp order.
+// Integer instructions (ALU pipe, half rate) are the next bound: 7 per word of 8 weights, about 40 per 512 bytes in all.
+// The first form, with 16-byte cp.async copies by all lanes, spent 72 there and took 20.8 us at 8192 x 8192.
 #include "common.cuh"
+#include "tcgen05.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -27,39 +33,32 @@ namespace prism_b200 {
 namespace {
 
 namespace w4 {
-constexpr int WARPS = 8;
+constexpr int WARPS = 16;
 constexpr int THREADS = 32 * WARPS;
-constexpr int ROWS = 32;                 // weight rows per item
+constexpr int ROWS = 32;                 // weight rows per warp
 constexpr int SLICE = 128;               // k per stage
+constexpr int COLS = 8;                  // rows of x per item: the columns of one MMA
 constexpr int W_BYTES = ROWS * SLICE / 2;
 constexpr int X_PITCH = SLICE * 2;
-constexpr int COLS = 8;                  // rows of x per item: the columns of one MMA
 constexpr int RED_PITCH = 36;            // a fragment's 8 x 4 places lie in 32 banks
-constexpr int RED_FLOATS = WARPS * COLS * RED_PITCH;
+constexpr int MAX_STAGES = 6;
 constexpr int MAX_EXPERTS = 1024;
+constexpr int RING_BYTES = 196608;
 
-// A stage: 32 weight rows of 64 bytes, then the rows of x of 256 bytes, in 16-byte pieces.  The pieces of a row are
-// permuted so that a step's reads lie in 32 different banks: 8 weight rows' words of one piece, and a quarter warp's two
-// rows of x with four pieces each.
-__device__ __forceinline__ int w_piece(int row, int piece) { return row * (SLICE / 2) + ((piece ^ ((row >> 1) & 3)) << 4); }
-__device__ __forceinline__ int x_piece(int row, int piece) { return W_BYTES + row * X_PITCH + ((piece ^ ((row & 1) << 2)) << 4); }
-
-struct Smem {
-    int stage, ring, bytes;              // ring: all warps' stages
-    __host__ __device__ Smem(int stages, int rows, int experts)
-        : stage(W_BYTES + (rows < COLS ? rows : COLS) * X_PITCH), ring(WARPS * stages * stage),
-          bytes(ring + RED_FLOATS * 4 + (3 * experts + 1) * 4) {}
+// Shared memory: rings (512-byte aligned), sums of the warps, barriers, flags, tables.
+struct Layout {
+    int xrows, stage, stages, red, bars, bytes;
+    __host__ __device__ Layout(int rows, int experts) {
+        xrows = rows < COLS ? rows : COLS;
+        stage = W_BYTES + (xrows * X_PITCH + 511) / 512 * 512;
+        stages = RING_BYTES / (WARPS * stage);
+        if (stages > MAX_STAGES) stages = MAX_STAGES;
+        red = WARPS * stages * stage;
+        bars = red + WARPS * xrows * RED_PITCH * 4;
+        bytes = 1024 + bars + WARPS * MAX_STAGES * 8 + 16 + (3 * experts + 1) * 4;
+    }
 };
 }  // namespace w4
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 template <typename T> struct W4Type;
 template <> struct W4Type<__nv_bfloat16> {
@@ -94,205 +93,242 @@ template <> struct W4Type<__half> {
 };
 
 struct W4Args {
-    const void* x;
-    long long ldx;
-    const uint8_t* q;
     const uint16_t* scales;
     const uint8_t* zeros;     // null: 8 everywhere
     const int* offsets;       // null: one matrix, all rows
     void* out;
     long long ldo;
     int rows, experts, n, k;
+    int split;                // warps that share 32 weight rows along k (a power of two)
     int aligned;              // a slice's scales (zeros) of a row can be read as one vector
 };
 
-struct Item {
-    int e, n0, r0, cols;
-};
+__device__ __forceinline__ void tma_load_w4(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_x(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
 
-// A warp's place in the sequence of (item, slice) pairs that its CTA works through; moves forward only.
+// A warp's place in the sequence of (item, slice) pairs that it works through; moves forward only.  An item is
+// 32 * (WARPS / split) weight rows of one expert and up to 8 of its rows of x; the items of one weight tile follow one
+// another, so that more than 8 rows find the weights in L2.
 struct Cursor {
     int t, s, e = 0;
-    Item item;
-    __device__ __forceinline__ void decode(const W4Args& a, const int* first, const int* last, const int* items, int n_tiles) {
-        while (items[e + 1] <= t) ++e;
-        const int in = t - items[e];
-        const int chunks = (last[e] - first[e] + w4::COLS - 1) / w4::COLS;   // chunks of one weight tile follow one another: L2
-        const int tile = in / chunks, chunk = in - tile * chunks;
-        item.e = e;
-        item.n0 = tile * w4::ROWS;
-        item.r0 = first[e] + chunk * w4::COLS;
-        item.cols = min(w4::COLS, last[e] - item.r0);
+    int n0, r0, cols;
+    __device__ __forceinline__ void decode(const W4Args& a, const int* first, const int* last, const int* items, int warp_row) {
+        const int tile_rows = w4::ROWS * (w4::WARPS / a.split);
+        int in = t, lo = 0, hi = a.rows;
+        if (a.offsets) {
+            while (items[e + 1] <= t) ++e;
+            in = t - items[e];
+            lo = first[e];
+            hi = last[e];
+        }
+        const int chunks = (hi - lo + w4::COLS - 1) / w4::COLS;
+        const int tile = chunks == 1 ? in : in / chunks, chunk = in - tile * chunks;
+        n0 = tile * tile_rows + warp_row * w4::ROWS;
+        r0 = lo + chunk * w4::COLS;
+        cols = min(w4::COLS, hi - r0);
     }
 };
 
-template <typename T, int G, bool Z, int STAGES>
-__global__ void __launch_bounds__(w4::THREADS, 2) gemv_w4_kernel(const W4Args a) {
+template <typename T, int G, bool Z>
+__global__ void __launch_bounds__(w4::THREADS, 1)
+gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     using namespace w4;
     using M = W4Type<T>;
     constexpr int PER = SLICE / G;          // groups per slice: 4, 2, 1
     constexpr int STEPS = G / 32;           // steps per group
-    extern __shared__ __align__(16) unsigned char smem[];
-    const Smem layout(STAGES, a.rows, a.experts);
-    float* red = reinterpret_cast<float*>(smem + layout.ring);
-    int* first = reinterpret_cast<int*>(red + RED_FLOATS);
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const Layout layout(a.rows, a.experts);
+    float* red = reinterpret_cast<float*>(smem + layout.red);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + layout.bars);
+    uint32_t* flags = reinterpret_cast<uint32_t*>(bars + WARPS * MAX_STAGES);
+    volatile uint32_t* abort_flag = flags;
+    volatile uint32_t* never_flag = flags + 1;
+    int* first = reinterpret_cast<int*>(flags + 4);
     int* last = first + a.experts;
     int* items = last + a.experts;          // [experts + 1]: first item of each expert
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
-    const int n_tiles = (a.n + ROWS - 1) / ROWS;
+    const int warp_row = warp / a.split, warp_k = warp % a.split;
+    const int tile_rows = ROWS * (WARPS / a.split);
+    const int n_tiles = (a.n + tile_rows - 1) / tile_rows;
     const int slices = (a.k + SLICE - 1) / SLICE;
     const int groups_row = a.k / G;
+    const int stages = layout.stages;
 
-    for (int e = threadIdx.x; e < a.experts; e += THREADS) {
-        const int lo = a.offsets ? min(max(a.offsets[e], 0), a.rows) : 0;
-        first[e] = lo;
-        last[e] = a.offsets ? min(max(a.offsets[e + 1], lo), a.rows) : a.rows;
+    uint64_t* full = bars + warp * MAX_STAGES;
+    if (lane == 0) {
+        for (int i = 0; i < stages; ++i) mbar_init(&full[i], 1);
+        if (warp == 0) *abort_flag = *never_flag = 0;
+        fence_barrier_init();
     }
-    __syncthreads();
-    if (warp == 0) {
-        int carry = 0;
-        for (int e0 = 0; e0 < a.experts; e0 += 32) {
-            const int e = e0 + lane;
-            const int n = e < a.experts ? (last[e] - first[e] + w4::COLS - 1) / w4::COLS * n_tiles : 0;
-            int incl = n;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= d) incl += up;
-            }
-            if (e < a.experts) items[e] = carry + incl - n;
-            carry += __shfl_sync(0xffffffffu, incl, 31);
+    int total;
+    if (a.offsets) {
+        for (int e = threadIdx.x; e < a.experts; e += THREADS) {
+            const int lo = min(max(a.offsets[e], 0), a.rows);
+            first[e] = lo;
+            last[e] = min(max(a.offsets[e + 1], lo), a.rows);
         }
-        if (lane == 0) items[a.experts] = carry;
+        __syncthreads();
+        if (warp == 0) {
+            int carry = 0;
+            for (int e0 = 0; e0 < a.experts; e0 += 32) {
+                const int e = e0 + lane;
+                const int n = e < a.experts ? (last[e] - first[e] + COLS - 1) / COLS * n_tiles : 0;
+                int incl = n;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, incl, d);
+                    if (lane >= d) incl += up;
+                }
+                if (e < a.experts) items[e] = carry + incl - n;
+                carry += __shfl_sync(0xffffffffu, incl, 31);
+            }
+            if (lane == 0) items[a.experts] = carry;
+        }
+        __syncthreads();
+        total = items[a.experts];
+    } else {
+        __syncthreads();
+        total = (a.rows + COLS - 1) / COLS * n_tiles;
     }
-    __syncthreads();
-    const int total = items[a.experts];
 
-    unsigned char* ring = smem + warp * STAGES * layout.stage;
-    const uint32_t ring_addr = smem_u32(ring);
+    unsigned char* ring = smem + warp * stages * layout.stage;
+    const uint32_t ring_addr = smem_u32(ring), full_addr = smem_u32(full);
+    const uint32_t stage_bytes = W_BYTES + layout.xrows * X_PITCH;
 
-    // ---- loads: one slice per call, in the order in which they are used ----
+    // ---- copies: one slice per call, in the order in which they are used ----
     Cursor load;
     load.t = blockIdx.x;
-    load.s = warp;
-    if (load.t < total) load.decode(a, first, last, items, n_tiles);
-    int load_slot = 0;
+    load.s = warp_k;
+    if (load.t < total) load.decode(a, first, last, items, warp_row);
+    int load_slot = 0, armed = 0;
     auto issue = [&] {
-        if (load.t < total && load.s < slices) {
-            const uint32_t dst = ring_addr + load_slot * layout.stage;
-            const int k0 = load.s * SLICE;
-            const int piece = lane & 3;                       // 16 bytes = 32 k
-            if (k0 + piece * 32 < a.k) {
-                const uint8_t* src = a.q + ((static_cast<size_t>(load.item.e) * a.n + load.item.n0 + g) * a.k + k0) / 2 + piece * 16;
-#pragma unroll
-                for (int i = 0; i < ROWS / 8; ++i)
-                    if (load.item.n0 + g + 8 * i < a.n)
-                        cp_async16(dst + w_piece(g + 8 * i, piece), src + static_cast<size_t>(i) * 4 * a.k);
-            }
-            const int xpiece = lane & 15;                     // 16 bytes = 8 k
-            if (k0 + xpiece * 8 < a.k) {
-                const T* src = static_cast<const T*>(a.x) + static_cast<size_t>(load.item.r0) * a.ldx + k0 + xpiece * 8;
-                for (int r = lane >> 4; r < load.item.cols; r += 2)
-                    cp_async16(dst + x_piece(r, xpiece), src + static_cast<size_t>(r) * a.ldx);
-            }
-            load.s += WARPS;
-            if (load.s >= slices) {
-                load.s = warp;
-                load.t += gridDim.x;
-                if (load.t < total) load.decode(a, first, last, items, n_tiles);
-            }
+        if (load.t >= total) return;
+        if (lane == 0) {
+            const uint32_t dst = ring_addr + load_slot * layout.stage, bar = full_addr + load_slot * 8;
+            mbar_arrive_expect_tx(&full[load_slot], stage_bytes);
+            tma_load_w4(dst, &map_w, load.s * (SLICE / 2), load.n0, load.e, bar);
+            tma_load_x(dst + W_BYTES, &map_x, load.s * SLICE, load.r0, bar);
         }
-        cp_async_commit();
-        load_slot = load_slot + 1 == STAGES ? 0 : load_slot + 1;
+        ++armed;
+        load_slot = load_slot + 1 == stages ? 0 : load_slot + 1;
+        load.s += a.split;
+        if (load.s >= slices) {
+            load.s = warp_k;
+            load.t += gridDim.x;
+            if (load.t < total) load.decode(a, first, last, items, warp_row);
+        }
     };
-    for (int i = 0; i < STAGES - 1; ++i) issue();
+    for (int i = 0; i < stages - 1; ++i) issue();
 
     // ---- scales and zeros of the next slice, in registers: rows g + 8 h, h = 0..3, PER groups each ----
     Cursor ahead;
     ahead.t = blockIdx.x;
-    ahead.s = warp;
-    if (ahead.t < total) ahead.decode(a, first, last, items, n_tiles);
-    uint16_t sc_next[4][PER];
-    uint8_t zr_next[4][PER];
+    ahead.s = warp_k;
+    const uint16_t* sc_row[4];
+    const uint8_t* zr_row[4];
+    auto rows_of = [&] {
+        ahead.decode(a, first, last, items, warp_row);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            const size_t at = (static_cast<size_t>(ahead.e) * a.n + min(ahead.n0 + g + 8 * h, a.n - 1)) * groups_row;
+            sc_row[h] = a.scales + at;
+            if (Z) zr_row[h] = a.zeros + at;
+        }
+    };
+    if (ahead.t < total) rows_of();
+    struct alignas(2 * PER) Scales { uint16_t v[PER]; };
+    struct alignas(PER) Zeros { uint8_t v[PER]; };
+    Scales sc_next[4];
+    Zeros zr_next[4];
     auto fetch = [&] {
-        if (ahead.t < total && ahead.s < slices) {
-            const int g0 = ahead.s * PER;
+        if (ahead.t >= total) return;
+        const int g0 = ahead.s * PER;
 #pragma unroll
-            for (int h = 0; h < 4; ++h) {
-                const int row = min(ahead.item.n0 + g + 8 * h, a.n - 1);
-                const size_t at = (static_cast<size_t>(ahead.item.e) * a.n + row) * groups_row + g0;
-                if (PER == 1 || a.aligned) {
-                    struct alignas(2 * PER) S { uint16_t v[PER]; };
-                    struct alignas(PER) B { uint8_t v[PER]; };
-                    const S s = *reinterpret_cast<const S*>(a.scales + at);
+        for (int h = 0; h < 4; ++h) {
+            if (PER == 1 || a.aligned) {
+                sc_next[h] = *reinterpret_cast<const Scales*>(sc_row[h] + g0);
+                if (Z) zr_next[h] = *reinterpret_cast<const Zeros*>(zr_row[h] + g0);
+            } else {
 #pragma unroll
-                    for (int p = 0; p < PER; ++p) sc_next[h][p] = s.v[p];
-                    if (Z) {
-                        const B z = *reinterpret_cast<const B*>(a.zeros + at);
-#pragma unroll
-                        for (int p = 0; p < PER; ++p) zr_next[h][p] = z.v[p];
-                    }
-                } else {
-#pragma unroll
-                    for (int p = 0; p < PER; ++p) {
-                        if (g0 + p < groups_row) {
-                            sc_next[h][p] = a.scales[at + p];
-                            if (Z) zr_next[h][p] = a.zeros[at + p];
-                        }
-                    }
+                for (int p = 0; p < PER; ++p) {   // no scale behind the row's last group: its products are zeros
+                    const bool there = g0 + p < groups_row;
+                    sc_next[h].v[p] = there ? sc_row[h][g0 + p] : 0;
+                    if (Z) zr_next[h].v[p] = there ? zr_row[h][g0 + p] : 0;
                 }
             }
-            ahead.s += WARPS;
-            if (ahead.s >= slices) {
-                ahead.s = warp;
-                ahead.t += gridDim.x;
-                if (ahead.t < total) ahead.decode(a, first, last, items, n_tiles);
-            }
+        }
+        ahead.s += a.split;
+        if (ahead.s >= slices) {
+            ahead.s = warp_k;
+            ahead.t += gridDim.x;
+            if (ahead.t < total) rows_of();
         }
     };
     fetch();
 
     Cursor at;
     int slot = 0;
+    uint32_t phase = 0;
+    bool timed_out = false;
+    // Offsets inside a stage that do not change: a lane's words of step 0 in rows g + 8 h (the swizzle of rows 8 apart is
+    // the same), and its piece of x.
+    const int w_at = g * (SLICE / 2) + c * 4, w_swizzle = ((g >> 1) & 3) << 4;
+    const int x_at = W_BYTES + g * X_PITCH + c * 16;
     for (at.t = blockIdx.x; at.t < total; at.t += gridDim.x) {
-        at.decode(a, first, last, items, n_tiles);
-        const int cols = at.item.cols;
+        at.decode(a, first, last, items, warp_row);
+        const int cols = at.cols;
         float sum[2][4];   // [16 weight rows][C fragment]
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[0][i] = sum[1][i] = 0.f;
 
-        for (int s = warp; s < slices; s += WARPS) {
-            cp_async_wait<STAGES - 2>();
+        for (int s = warp_k; s < slices; s += a.split) {
+            if (!timed_out && !__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], phase, abort_flag))) {
+                timed_out = true;   // go on to the block's barriers without waiting for copies again
+                *abort_flag = 1;
+                if (lane == 0) raise_device_status(DEV_GEMV_PIPE_TIMEOUT);
+            }
             __syncwarp();
-            issue();   // into the slot consumed one iteration ago
+            if (!timed_out) issue();   // into the slot consumed one iteration ago
             float sc[4][PER], zr[4][PER];
 #pragma unroll
             for (int h = 0; h < 4; ++h)
 #pragma unroll
                 for (int p = 0; p < PER; ++p) {
-                    sc[h][p] = M::to_f32(sc_next[h][p]);
-                    zr[h][p] = Z ? 16.f + static_cast<float>(zr_next[h][p]) : 24.f;
+                    sc[h][p] = M::to_f32(sc_next[h].v[p]);
+                    zr[h][p] = Z ? -16.f - static_cast<float>(zr_next[h].v[p]) : -24.f;
                 }
             fetch();
             const unsigned char* here = ring + slot * layout.stage;
-            slot = slot + 1 == STAGES ? 0 : slot + 1;
-            const int groups_here = min(PER, (a.k - s * SLICE) / G);
+            if (++slot == stages) {
+                slot = 0;
+                phase ^= 1u;
+            }
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
-                if (p >= groups_here) break;
                 float acc[2][4], ones[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = ones[i] = 0.f;
 #pragma unroll
                 for (int st = 0; st < STEPS; ++st) {
                     const int step = p * STEPS + st;
+                    const unsigned char* words = here + w_at + ((step << 4) ^ w_swizzle);
                     uint32_t w[4];
 #pragma unroll
-                    for (int h = 0; h < 4; ++h)
-                        w[h] = *reinterpret_cast<const uint32_t*>(here + w_piece(g + 8 * h, step) + c * 4);
+                    for (int h = 0; h < 4; ++h) w[h] = *reinterpret_cast<const uint32_t*>(words + 8 * h * (SLICE / 2));
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    if (g < cols) v = *reinterpret_cast<const uint4*>(here + x_piece(g, step * 4 + c));
+                    if (g < cols) v = *reinterpret_cast<const uint4*>(here + x_at + step * 64);
                     const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
                     const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
                     M::mma(ones, M::ONES, M::ONES, M::ONES, M::ONES, b0, b1);
@@ -310,12 +346,12 @@ __global__ void __launch_bounds__(w4::THREADS, 2) gemv_w4_kernel(const W4Args a)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int h = 2 * m + (i >> 1);
-                        sum[m][i] = fmaf(sc[h][p], fmaf(-zr[h][p], ones[i & 1], acc[m][i]), sum[m][i]);
+                        sum[m][i] = fmaf(sc[h][p], fmaf(zr[h][p], ones[i & 1], acc[m][i]), sum[m][i]);
                     }
             }
         }
 
-        float* part = red + warp * COLS * RED_PITCH;
+        float* part = red + warp * layout.xrows * RED_PITCH;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -324,23 +360,43 @@ __global__ void __launch_bounds__(w4::THREADS, 2) gemv_w4_kernel(const W4Args a)
                 if (col < cols) part[col * RED_PITCH + m * 16 + (i >> 1) * 8 + g] = sum[m][i];
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < cols * ROWS; i += THREADS) {
-            const int col = i / ROWS, row = i % ROWS;
-            if (at.item.n0 + row >= a.n) continue;
-            const float* p = red + col * RED_PITCH + row;
+        const int n_first = at.n0 - warp_row * ROWS;
+        for (int i = threadIdx.x; i < cols * tile_rows; i += THREADS) {
+            const int col = i / tile_rows, row = i - col * tile_rows;
+            if (n_first + row >= a.n) continue;
+            const float* p = red + ((row / ROWS) * a.split * layout.xrows + col) * RED_PITCH + row % ROWS;
             float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) v += p[w * COLS * RED_PITCH];
-            static_cast<T*>(a.out)[static_cast<size_t>(at.item.r0 + col) * a.ldo + at.item.n0 + row] = M::from_f32(v);
+            for (int w = 0; w < a.split; ++w) v += p[w * layout.xrows * RED_PITCH];
+            static_cast<T*>(a.out)[static_cast<size_t>(at.r0 + col) * a.ldo + n_first + row] = M::from_f32(v);
         }
         __syncthreads();   // the next item's sums go to the same place
     }
-    cp_async_wait<0>();
+    if (timed_out && lane == 0) {
+        // Unwind: let copies already in flight land before shared memory is released.
+        for (int i = 0; i < stages && i < armed; ++i) {
+            const int behind = armed - 1 - i;   // the behind-th copy went to slot behind % stages, phase behind / stages
+            mbar_wait_bounded(&full[behind % stages], (behind / stages) & 1, never_flag, 2000000ull);
+        }
+    }
 }
 
-template <typename T, int G, bool Z, int STAGES>
-int launch_w4(const W4Args& a, long long most_items, cudaStream_t s) {
-    auto kern = gemv_w4_kernel<T, G, Z, STAGES>;
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+// Weights as bytes [experts][n][k / 2], boxes of 64 bytes x 32 rows; x as rows of 16-bit elements, boxes of 128 x xrows.
+int w4_maps(CUtensorMap* map_w, CUtensorMap* map_x, const W4Args& a, const uint8_t* q, const void* x, long long ldx, int xrows) {
+    const cuuint64_t wdims[3] = {static_cast<cuuint64_t>(a.k) / 2, static_cast<cuuint64_t>(a.n), static_cast<cuuint64_t>(a.experts)};
+    const cuuint64_t wstrides[2] = {static_cast<cuuint64_t>(a.k) / 2, static_cast<cuuint64_t>(a.n) * a.k / 2};
+    const cuuint32_t wbox[3] = {w4::SLICE / 2, w4::ROWS, 1};
+    if (int rc = encode_tensor_map(map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, q, wdims, wstrides, wbox, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+    const cuuint64_t xdims[2] = {static_cast<cuuint64_t>(a.k), static_cast<cuuint64_t>(a.rows)};
+    const cuuint64_t xstrides[1] = {static_cast<cuuint64_t>(ldx) * 2};
+    const cuuint32_t xbox[2] = {w4::SLICE, static_cast<cuuint32_t>(xrows)};
+    return encode_tensor_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, x, xdims, xstrides, xbox, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+template <typename T, int G, bool Z>
+int launch_w4(W4Args a, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
+    auto kern = gemv_w4_kernel<T, G, Z>;
     static std::mutex mu;
     static int sm_count[64] = {};
     int dev = 0, sms = 0;
@@ -349,41 +405,44 @@ int launch_w4(const W4Args& a, long long most_items, cudaStream_t s) {
         std::lock_guard<std::mutex> lk(mu);
         const bool cacheable = dev >= 0 && dev < 64;
         if (!cacheable || !sm_count[dev]) {
-            PRISM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                w4::Smem(STAGES, w4::COLS, w4::MAX_EXPERTS).bytes));
+            PRISM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
             PRISM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
             if (cacheable) sm_count[dev] = sms;
         } else {
             sms = sm_count[dev];
         }
     }
-    const long long cap = 2LL * sms;   // resident CTAs, by registers and shared memory
-    const int grid = static_cast<int>(most_items < cap ? most_items : cap);
-    kern<<<grid, w4::THREADS, w4::Smem(STAGES, a.rows, a.experts).bytes, s>>>(a);
+    // Warps per 32 weight rows: as many as leave each four slices of k, more where the rows alone do not fill the SMs.
+    const int slices = (a.k + w4::SLICE - 1) / w4::SLICE;
+    const long long groups = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
+    auto most = [&](int split) {
+        const int tile_rows = w4::ROWS * (w4::WARPS / split);
+        return (a.n + tile_rows - 1LL) / tile_rows * (a.rows / w4::COLS + groups);
+    };
+    int split = 1;
+    while (split < w4::WARPS && slices >= 8 * split) split *= 2;
+    while (split < w4::WARPS && slices >= 2 * split && most(split) < sms) split *= 2;
+    a.split = split;
+    const w4::Layout layout(a.rows, a.experts);
+    CUtensorMap map_w, map_x;
+    if (int rc = w4_maps(&map_w, &map_x, a, q, x, ldx, layout.xrows)) return rc;
+    const int grid = static_cast<int>(most(split) < sms ? most(split) : sms);
+    kern<<<grid, w4::THREADS, layout.bytes, s>>>(a, map_w, map_x);
     PRISM_CUDA_TRY(cudaGetLastError());
     count_launch();
     return PRISM_B200_OK;
 }
 
-// Stages of a warp's ring: four with up to four rows of x, three with more, so that two CTAs fit an SM.
-template <typename T, int G, bool Z>
-int launch_w4_stages(const W4Args& a, cudaStream_t s) {
-    const long long tiles = (a.n + w4::ROWS - 1) / w4::ROWS;
-    const long long groups = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-    const long long most = tiles * (a.rows / w4::COLS + groups);
-    return a.rows <= 4 ? launch_w4<T, G, Z, 4>(a, most, s) : launch_w4<T, G, Z, 3>(a, most, s);
-}
-
 template <typename T, int G>
-int launch_w4_zeros(const W4Args& a, cudaStream_t s) {
-    return a.zeros ? launch_w4_stages<T, G, true>(a, s) : launch_w4_stages<T, G, false>(a, s);
+int launch_w4_zeros(const W4Args& a, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
+    return a.zeros ? launch_w4<T, G, true>(a, q, x, ldx, s) : launch_w4<T, G, false>(a, q, x, ldx, s);
 }
 
 template <typename T>
-int launch_w4_group(const W4Args& a, int group, cudaStream_t s) {
-    if (group == 32) return launch_w4_zeros<T, 32>(a, s);
-    if (group == 64) return launch_w4_zeros<T, 64>(a, s);
-    return launch_w4_zeros<T, 128>(a, s);
+int launch_w4_group(const W4Args& a, int group, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
+    if (group == 32) return launch_w4_zeros<T, 32>(a, q, x, ldx, s);
+    if (group == 64) return launch_w4_zeros<T, 64>(a, q, x, ldx, s);
+    return launch_w4_zeros<T, 128>(a, q, x, ldx, s);
 }
 
 }  // namespace
@@ -415,7 +474,8 @@ extern "C" int prism_b200_gemv_w4(int dtype, int rows, int experts, int n, int k
         return set_error(PRISM_B200_ERR_MISALIGNED, "gemv_w4: scales and out must be 2-byte aligned");
     const int per = 128 / group;
     const bool aligned = k % 128 == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * per) == 0 && reinterpret_cast<uintptr_t>(zeros) % per == 0;
-    const W4Args a{x, ldx, q, static_cast<const uint16_t*>(scales), zeros, offsets, out, ldo, rows, experts, n, k, aligned ? 1 : 0};
+    if (int rc = bind_status_word()) return rc;
+    const W4Args a{static_cast<const uint16_t*>(scales), zeros, offsets, out, ldo, rows, experts, n, k, 1, aligned ? 1 : 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return dtype == PRISM_B200_BF16 ? launch_w4_group<__nv_bfloat16>(a, group, s) : launch_w4_group<__half>(a, group, s);
+    return dtype == PRISM_B200_BF16 ? launch_w4_group<__nv_bfloat16>(a, group, q, x, ldx, s) : launch_w4_group<__half>(a, group, q, x, ldx, s);
 }

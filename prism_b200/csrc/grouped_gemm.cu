@@ -667,38 +667,12 @@ grouped_gemm_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap map
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int encode(CUtensorMap* out, int rank, const void* ptr, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
-    static std::mutex mu;
-    static EncodeTiledFn fn = nullptr;
-    {
-        std::lock_guard<std::mutex> lk(mu);
-        if (!fn) {
-            void* p = nullptr;
-            cudaDriverEntryPointQueryResult q;
-            cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-            if (e != cudaSuccess || !p || q != cudaDriverEntryPointSuccess)
-                return set_error(PRISM_B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        }
-    }
-    const cuuint32_t estr[3] = {1, 1, 1};
-    const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(ptr), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return set_error(PRISM_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
-    return PRISM_B200_OK;
-}
-
 // Rows of activations: width contiguous, 64 x 64 boxes.
 int rows_map(CUtensorMap* out, const void* ptr, long long rows, int width, long long ld) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
     const cuuint32_t box[2] = {64, 64};
-    return encode(out, 2, ptr, dims, strides, box);
+    return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // Weights [experts][n][k]: boxes of 64 k and box_n rows of one expert.
@@ -706,7 +680,7 @@ int weights_map(CUtensorMap* out, const void* ptr, int experts, int n, int k, in
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(experts)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(k) * 2, static_cast<cuuint64_t>(n) * k * 2};
     const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_n), 1};
-    return encode(out, 3, ptr, dims, strides, box);
+    return encode_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int MODE, typename Out, int NB>

@@ -133,4 +133,8 @@ __device__ __forceinline__ void drain_pair_loads(uint64_t* full_bar, int stage, 
     }
 }
 
+// A tiled tensor map without cached state (api.cu): dims[rank] and box[rank] in elements, strides[rank - 1] in bytes.
+int encode_tensor_map(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* ptr, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle);
+
 }  // namespace prism_b200
