@@ -7,22 +7,21 @@
 // 23 bytes (46 weights) per clock to keep up with HBM.
 //   * Products and sums are mma.sync m16n8k16 with fp32 accumulators: 16 weight rows x 16 k against up to 8 rows of x.
 //     tcgen05 would want the converted weights in shared memory, a round trip of four times the bytes read here.
-//   * A nibble becomes an operand by one shift and one LOP3: put into the four top bits of the mantissa of 16.0 it
-//     makes 16 + q, exactly, in bf16 and fp16 alike.  The 16 + z is taken off afterwards, once per group, in fp32:
+//   * A nibble becomes an operand by one shift and one LOP3: put into the mantissa of 16.0 (bf16) or 64.0 (fp16) it makes
+//     16 + q or 64 + q, exactly.  The base and z are taken off afterwards, once per group, in fp32:
 //     sum (q - z) x = sum (16 + q) x - (16 + z) * sum x, with sum x from one more MMA whose weight operand is all ones.
-//     The larger terms cost at most 3 bits of the fp32 accumulator's 24, far below the rounding of y to 16 bits.
+//     The larger terms cost 3 or 5 bits of the fp32 accumulator's 24, far below the rounding of y to 16 bits.
 //   * A 32-bit word holds 8 consecutive k; the MMA's order of k is free as long as both operands follow it, so the
 //     pairs are (k, k + 4) as the masks deliver them, and x is brought into that order by four PRMTs per 8 values.
-//   * The four lanes of a quad take the four words of 32 consecutive k, so a group of 32, 64 or 128 is 1, 2 or 4 steps
-//     and its sum is complete in the accumulator when its scale is applied (fp32).
-//   * A warp takes 32 weight rows and a share of k in slices of 128; `split` warps share the same rows, so that long rows
-//     are split and short ones are not (four slices per warp where there are enough).  A slice (2 KB of weights, and its
-//     256 bytes of each row of x) is two TMA copies into a ring of the warp's own, issued by one lane; the ring runs on
-//     across work items, so no block barrier is between a copy and its use.  The copies' 64-byte swizzle keeps a step's
-//     reads free of bank conflicts, and what lies outside the matrices arrives as zeros.
-//   * The warps' sums meet in shared memory once per item, added in warp order.
-// Integer instructions (ALU pipe, half rate) are the next bound: 7 per word of 8 weights, about 40 per 512 bytes in all.
-// The first form, with 16-byte cp.async copies by all lanes, spent 72 there and took 20.8 us at 8192 x 8192.
+//   * The four lanes of a quad take one, two or four consecutive words each, 32, 64 or 128 k together: a group, whose sum is
+//     then complete in the accumulator when its scale is applied (fp32).  A group of 128 is one 16-byte read per row.
+//   * A team of 1 to 16 warps takes 32 weight rows, each warp a range of k in slices of 128.  A slice (64 bytes of each
+//     weight row, 256 of each row of x) is two TMA copies into a ring of the warp's own, issued by one lane; the ring runs
+//     on across work items, so no barrier is between a copy and its use.  The copies' 64-byte swizzle keeps the reads free
+//     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
+//     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
+//   * The team's sums meet in shared memory once per item, added in warp order.
+// Integer instructions (ALU pipe, half rate) are the next bound: 7 per word of 8 weights in bf16, 5 in fp16.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -34,63 +33,103 @@ namespace {
 
 namespace w4 {
 constexpr int WARPS = 16;
+constexpr int ROWS = 32;                 // weight rows per item
 constexpr int THREADS = 32 * WARPS;
-constexpr int ROWS = 32;                 // weight rows per warp
 constexpr int SLICE = 128;               // k per stage
 constexpr int COLS = 8;                  // rows of x per item: the columns of one MMA
-constexpr int W_BYTES = ROWS * SLICE / 2;
 constexpr int X_PITCH = SLICE * 2;
-constexpr int RED_PITCH = 36;            // a fragment's 8 x 4 places lie in 32 banks
+constexpr int W_BYTES = ROWS * SLICE / 2;
+constexpr int RED_PITCH = ROWS + 4;      // a fragment's 8 x 4 places lie in 32 banks
+constexpr int BLOCK = 8;                 // groups whose scales are copied at a time
+constexpr int SC_BYTES = ROWS * BLOCK * 3;   // a block: 16 bytes of scales per row, then 8 bytes of zero points per row
 constexpr int MAX_STAGES = 6;
 constexpr int MAX_EXPERTS = 1024;
-constexpr int RING_BYTES = 196608;
+constexpr int SMEM_BYTES = 232448;
 
-// Shared memory: rings (512-byte aligned), sums of the warps, barriers, flags, tables.
+// Shared memory: rings (512-byte aligned), scales (two blocks per warp), sums of the warps (two sets), barriers, flags, tables.
 struct Layout {
-    int xrows, stage, stages, red, bars, bytes;
+    int xrows, stage, stages, red_floats, scales, red, bars, bytes;
     __host__ __device__ Layout(int rows, int experts) {
         xrows = rows < COLS ? rows : COLS;
         stage = W_BYTES + (xrows * X_PITCH + 511) / 512 * 512;
-        stages = RING_BYTES / (WARPS * stage);
+        red_floats = xrows * RED_PITCH;
+        const int rest = 1024 + WARPS * (2 * SC_BYTES + 2 * red_floats * 4 + MAX_STAGES * 8) + 16 + (experts > 1 ? (3 * experts + 1) * 4 : 16);
+        stages = (SMEM_BYTES - rest) / (WARPS * stage);
         if (stages > MAX_STAGES) stages = MAX_STAGES;
-        red = WARPS * stages * stage;
-        bars = red + WARPS * xrows * RED_PITCH * 4;
-        bytes = 1024 + bars + WARPS * MAX_STAGES * 8 + 16 + (3 * experts + 1) * 4;
+        scales = WARPS * stages * stage;
+        red = scales + WARPS * 2 * SC_BYTES;
+        bars = red + WARPS * 2 * red_floats * 4;
+        bytes = rest + scales;
     }
 };
 }  // namespace w4
 
+// (a & b) | c in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+
 template <typename T> struct W4Type;
 template <> struct W4Type<__nv_bfloat16> {
     static constexpr uint32_t ONES = 0x3F803F80u;
-    // nibble i of the word's two halves -> (16 + q) twice; 16.0 is 0x4180, the mantissa's top four bits are bits 3-6
+    static constexpr float BASE = 16.f;
+    // nibble i of the word's two halves -> (16 + q) twice: 16.0 is 0x4180, the mantissa's top four bits are bits 3-6
     template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-        const uint32_t s = I == 0 ? w << 3 : w >> (4 * I - 3);
-        return (s & 0x00780078u) | 0x41804180u;
+        const uint32_t s = I == 0 ? w * 8u : w >> (4 * I - 3);
+        return and_or(s, 0x00780078u, 0x41804180u);
     }
+    // d = a * b + d, or a * b where FIRST (no registers to clear before a group's first step)
+    template <bool FIRST>
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        if constexpr (FIRST) {
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+        } else {
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        }
     }
     static __device__ __forceinline__ float to_f32(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
     static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct W4Type<__half> {
     static constexpr uint32_t ONES = 0x3C003C00u;
-    // 16.0 is 0x4C00, the mantissa's top four bits are bits 6-9
+    static constexpr float BASE = 64.f;
+    // (64 + q) twice: 64.0 is 0x5400, and a nibble on bits 4-7 of its ten-bit mantissa counts in ones; left shifts are
+    // multiplications (FMA pipe), so a word takes one shift and four LOP3
     template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-        const uint32_t s = I < 2 ? w << (6 - 4 * I) : w >> (4 * I - 6);
-        return (s & 0x03C003C0u) | 0x4C004C00u;
+        const uint32_t t = I < 2 ? w : w >> 8;
+        return and_or(I & 1 ? t : t * 16u, 0x00F000F0u, 0x54005400u);
     }
+    // d = a * b + d, or a * b where FIRST (no registers to clear before a group's first step)
+    template <bool FIRST>
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        if constexpr (FIRST) {
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+        } else {
+            asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        }
     }
     static __device__ __forceinline__ float to_f32(uint16_t v) { return __half2float(__ushort_as_half(v)); }
     static __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 };
+
+// cp.async of 16 bytes past L1, of 8 bytes, and the wait for all of a thread's copies.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 struct W4Args {
     const uint16_t* scales;
@@ -99,8 +138,8 @@ struct W4Args {
     void* out;
     long long ldo;
     int rows, experts, n, k;
-    int split;                // warps that share 32 weight rows along k (a power of two)
-    int aligned;              // a slice's scales (zeros) of a row can be read as one vector
+    int split;                // warps of a team (a power of two)
+    int aligned;              // blocks of eight scales (zeros) can be copied as 16 (8) bytes
 };
 
 __device__ __forceinline__ void tma_load_w4(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
@@ -116,14 +155,12 @@ __device__ __forceinline__ void tma_load_x(uint32_t dst, const CUtensorMap* map,
         : "memory");
 }
 
-// A warp's place in the sequence of (item, slice) pairs that it works through; moves forward only.  An item is
-// 32 * (WARPS / split) weight rows of one expert and up to 8 of its rows of x; the items of one weight tile follow one
-// another, so that more than 8 rows find the weights in L2.
-struct Cursor {
-    int t, s, e = 0;
+// An item: 32 weight rows of one expert and up to 8 of its rows of x.  The items of one weight tile follow one another, so
+// that more than 8 rows find the weights in L2.  The walk over the experts only moves forward.
+struct Item {
+    int t, e = 0;
     int n0, r0, cols;
-    __device__ __forceinline__ void decode(const W4Args& a, const int* first, const int* last, const int* items, int warp_row) {
-        const int tile_rows = w4::ROWS * (w4::WARPS / a.split);
+    __device__ __forceinline__ void decode(const W4Args& a, const int* first, const int* last, const int* items) {
         int in = t, lo = 0, hi = a.rows;
         if (a.offsets) {
             while (items[e + 1] <= t) ++e;
@@ -133,11 +170,17 @@ struct Cursor {
         }
         const int chunks = (hi - lo + w4::COLS - 1) / w4::COLS;
         const int tile = chunks == 1 ? in : in / chunks, chunk = in - tile * chunks;
-        n0 = tile * tile_rows + warp_row * w4::ROWS;
+        n0 = tile * w4::ROWS;
         r0 = lo + chunk * w4::COLS;
         cols = min(w4::COLS, hi - r0);
     }
 };
+
+// Barrier of the warps of team `team` (named barrier team + 1).
+__device__ __forceinline__ void team_sync(int team, int threads) {
+    __syncwarp();
+    if (threads > 32) asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
+}
 
 template <typename T, int G, bool Z>
 __global__ void __launch_bounds__(w4::THREADS, 1)
@@ -145,7 +188,8 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
     using namespace w4;
     using M = W4Type<T>;
     constexpr int PER = SLICE / G;          // groups per slice: 4, 2, 1
-    constexpr int STEPS = G / 32;           // steps per group
+    constexpr int STEPS = G / 32;           // steps per group, and consecutive words per lane
+    constexpr int RUN = BLOCK / PER;        // slices per block of scales
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const Layout layout(a.rows, a.experts);
@@ -159,10 +203,11 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
     int* items = last + a.experts;          // [experts + 1]: first item of each expert
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
-    const int warp_row = warp / a.split, warp_k = warp % a.split;
-    const int tile_rows = ROWS * (WARPS / a.split);
-    const int n_tiles = (a.n + tile_rows - 1) / tile_rows;
+    const int team = warp / a.split, warp_k = warp % a.split, teams = WARPS / a.split, team_threads = 32 * a.split;
+    const int n_tiles = (a.n + ROWS - 1) / ROWS;
     const int slices = (a.k + SLICE - 1) / SLICE;
+    const int per_warp = (slices + a.split - 1) / a.split;
+    const int s_first = warp_k * per_warp, s_last = min(slices, s_first + per_warp);   // may be empty
     const int groups_row = a.k / G;
     const int stages = layout.stages;
 
@@ -202,156 +247,159 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
         __syncthreads();
         total = (a.rows + COLS - 1) / COLS * n_tiles;
     }
+    const int t_first = blockIdx.x * teams + team, t_step = gridDim.x * teams;
+    const int t_end = s_first < s_last ? total : 0;   // for the copies: a warp without slices has none
 
     unsigned char* ring = smem + warp * stages * layout.stage;
     const uint32_t ring_addr = smem_u32(ring), full_addr = smem_u32(full);
     const uint32_t stage_bytes = W_BYTES + layout.xrows * X_PITCH;
 
     // ---- copies: one slice per call, in the order in which they are used ----
-    Cursor load;
-    load.t = blockIdx.x;
-    load.s = warp_k;
-    if (load.t < total) load.decode(a, first, last, items, warp_row);
+    Item load;
+    load.t = t_first;
+    int load_s = s_first;
+    if (load.t < t_end) load.decode(a, first, last, items);
     int load_slot = 0, armed = 0;
     auto issue = [&] {
-        if (load.t >= total) return;
+        if (load.t >= t_end) return;
         if (lane == 0) {
             const uint32_t dst = ring_addr + load_slot * layout.stage, bar = full_addr + load_slot * 8;
             mbar_arrive_expect_tx(&full[load_slot], stage_bytes);
-            tma_load_w4(dst, &map_w, load.s * (SLICE / 2), load.n0, load.e, bar);
-            tma_load_x(dst + W_BYTES, &map_x, load.s * SLICE, load.r0, bar);
+            tma_load_w4(dst, &map_w, load_s * (SLICE / 2), load.n0, load.e, bar);
+            tma_load_x(dst + W_BYTES, &map_x, load_s * SLICE, load.r0, bar);
         }
         ++armed;
         load_slot = load_slot + 1 == stages ? 0 : load_slot + 1;
-        load.s += a.split;
-        if (load.s >= slices) {
-            load.s = warp_k;
-            load.t += gridDim.x;
-            if (load.t < total) load.decode(a, first, last, items, warp_row);
+        if (++load_s == s_last) {
+            load_s = s_first;
+            load.t += t_step;
+            if (load.t < t_end) load.decode(a, first, last, items);
         }
     };
     for (int i = 0; i < stages - 1; ++i) issue();
 
-    // ---- scales and zeros of the next slice, in registers: rows g + 8 h, h = 0..3, PER groups each ----
-    Cursor ahead;
-    ahead.t = blockIdx.x;
-    ahead.s = warp_k;
-    const uint16_t* sc_row[4];
-    const uint8_t* zr_row[4];
-    auto rows_of = [&] {
-        ahead.decode(a, first, last, items, warp_row);
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const size_t at = (static_cast<size_t>(ahead.e) * a.n + min(ahead.n0 + g + 8 * h, a.n - 1)) * groups_row;
-            sc_row[h] = a.scales + at;
-            if (Z) zr_row[h] = a.zeros + at;
-        }
-    };
-    if (ahead.t < total) rows_of();
-    struct alignas(2 * PER) Scales { uint16_t v[PER]; };
-    struct alignas(PER) Zeros { uint8_t v[PER]; };
-    Scales sc_next[4];
-    Zeros zr_next[4];
-    auto fetch = [&] {
-        if (ahead.t >= total) return;
-        const int g0 = ahead.s * PER;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            if (PER == 1 || a.aligned) {
-                sc_next[h] = *reinterpret_cast<const Scales*>(sc_row[h] + g0);
-                if (Z) zr_next[h] = *reinterpret_cast<const Zeros*>(zr_row[h] + g0);
-            } else {
-#pragma unroll
-                for (int p = 0; p < PER; ++p) {   // no scale behind the row's last group: its products are zeros
-                    const bool there = g0 + p < groups_row;
-                    sc_next[h].v[p] = there ? sc_row[h][g0 + p] : 0;
-                    if (Z) zr_next[h].v[p] = there ? zr_row[h][g0 + p] : 0;
-                }
+    // ---- scales and zeros, a block of eight groups per call: lane l copies row l ----
+    unsigned char* blocks = smem + layout.scales + warp * 2 * SC_BYTES;
+    const uint32_t blocks_addr = smem_u32(blocks);
+    Item ahead;
+    ahead.t = t_first;
+    int ahead_s = s_first;      // first slice of the block to be copied
+    int copies = 0;
+    if (ahead.t < t_end) ahead.decode(a, first, last, items);
+    auto copy_scales = [&] {
+        if (ahead.t >= t_end) return;
+        const int g0 = ahead_s * PER / BLOCK * BLOCK;
+        const size_t at = (static_cast<size_t>(ahead.e) * a.n + min(ahead.n0 + lane, a.n - 1)) * groups_row + g0;
+        const int into = (copies & 1) * SC_BYTES;
+        if (a.aligned) {
+            cp_async16(blocks_addr + into + lane * 16, a.scales + at);
+            if (Z) cp_async8(blocks_addr + into + ROWS * 16 + lane * 8, a.zeros + at);
+        } else {
+            uint16_t* sc = reinterpret_cast<uint16_t*>(blocks + into) + lane * BLOCK;
+            uint8_t* zr = blocks + into + ROWS * 16 + lane * BLOCK;
+            for (int i = 0; i < BLOCK; ++i) {   // no scale behind the row's last group: its products are zeros
+                const bool there = g0 + i < groups_row;
+                sc[i] = there ? a.scales[at + i] : 0;
+                if (Z) zr[i] = there ? a.zeros[at + i] : 0;
             }
         }
-        ahead.s += a.split;
-        if (ahead.s >= slices) {
-            ahead.s = warp_k;
-            ahead.t += gridDim.x;
-            if (ahead.t < total) rows_of();
+        ++copies;
+        ahead_s = (ahead_s / RUN + 1) * RUN;
+        if (ahead_s >= s_last) {
+            ahead_s = s_first;
+            ahead.t += t_step;
+            if (ahead.t < t_end) ahead.decode(a, first, last, items);
         }
     };
-    fetch();
+    copy_scales();
 
-    Cursor at;
-    int slot = 0;
+    Item at;
+    int slot = 0, set = 0, block = 0;
     uint32_t phase = 0;
     bool timed_out = false;
-    // Offsets inside a stage that do not change: a lane's words of step 0 in rows g + 8 h (the swizzle of rows 8 apart is
-    // the same), and its piece of x.
-    const int w_at = g * (SLICE / 2) + c * 4, w_swizzle = ((g >> 1) & 3) << 4;
-    const int x_at = W_BYTES + g * X_PITCH + c * 16;
-    for (at.t = blockIdx.x; at.t < total; at.t += gridDim.x) {
-        at.decode(a, first, last, items, warp_row);
+    // Where a lane reads in a stage: its words of row g (rows 8 apart have the same swizzle), its pieces of x.
+    const int w_row = g * (SLICE / 2), w_swizzle = (g >> 1) & 3;
+    const int x_row = W_BYTES + g * X_PITCH;
+    for (at.t = t_first; at.t < total; at.t += t_step) {
+        at.decode(a, first, last, items);
         const int cols = at.cols;
         float sum[2][4];   // [16 weight rows][C fragment]
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[0][i] = sum[1][i] = 0.f;
 
-        for (int s = warp_k; s < slices; s += a.split) {
-            if (!timed_out && !__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], phase, abort_flag))) {
-                timed_out = true;   // go on to the block's barriers without waiting for copies again
-                *abort_flag = 1;
-                if (lane == 0) raise_device_status(DEV_GEMV_PIPE_TIMEOUT);
-            }
+        for (int s = s_first; s < s_last;) {
+            // A block of scales: the copy made one block ago has landed, the next one starts.
+            cp_async_wait_all();
             __syncwarp();
-            if (!timed_out) issue();   // into the slot consumed one iteration ago
-            float sc[4][PER], zr[4][PER];
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
+            const unsigned char* sc_block = blocks + (block & 1) * SC_BYTES;
+            ++block;
+            copy_scales();
+            const int run_last = min(s_last, (s / RUN + 1) * RUN);
+            for (; s < run_last; ++s) {
+                if (!timed_out && !__all_sync(0xffffffffu, mbar_wait_bounded(&full[slot], phase, abort_flag))) {
+                    timed_out = true;   // go on to the team's barriers without waiting for copies again
+                    *abort_flag = 1;
+                    if (lane == 0) raise_device_status(DEV_GEMV_PIPE_TIMEOUT);
+                }
+                __syncwarp();
+                if (!timed_out) issue();   // into the slot consumed one iteration ago
+                const unsigned char* here = ring + slot * layout.stage;
+                if (++slot == stages) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+                const unsigned char* sc_slice = sc_block + g * 16 + (s % RUN) * (PER * 2);
+                const unsigned char* zr_slice = sc_block + ROWS * 16 + g * 8 + (s % RUN) * PER;
 #pragma unroll
                 for (int p = 0; p < PER; ++p) {
-                    sc[h][p] = M::to_f32(sc_next[h].v[p]);
-                    zr[h][p] = Z ? -16.f - static_cast<float>(zr_next[h].v[p]) : -24.f;
-                }
-            fetch();
-            const unsigned char* here = ring + slot * layout.stage;
-            if (++slot == stages) {
-                slot = 0;
-                phase ^= 1u;
-            }
+                    // A lane's STEPS consecutive words in rows g, g + 8, g + 16, g + 24.
+                    struct alignas(4 * STEPS) Words { uint32_t v[STEPS]; };
+                    Words w[4];
+                    const int byte = p * (G / 2) + c * (4 * STEPS);   // in the row's 64
+                    const unsigned char* words = here + w_row + ((((byte >> 4) ^ w_swizzle) << 4) | (byte & 15));
 #pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                float acc[2][4], ones[4];
+                    for (int h = 0; h < 4; ++h) w[h] = *reinterpret_cast<const Words*>(words + 8 * h * (SLICE / 2));
+                    float acc[2][4], ones[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = ones[i] = 0.f;
+                    for (int st = 0; st < STEPS; ++st) {
+                        uint4 v = make_uint4(0, 0, 0, 0);
+                        if (g < cols) v = *reinterpret_cast<const uint4*>(here + x_row + (p * G + (c * STEPS + st) * 8) * 2);
+                        const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
+                        const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
+                        if (st == 0) M::template mma<true>(ones, M::ONES, M::ONES, M::ONES, M::ONES, b0, b1);
+                        else M::template mma<false>(ones, M::ONES, M::ONES, M::ONES, M::ONES, b0, b1);
+                        M::template mma<false>(ones, M::ONES, M::ONES, M::ONES, M::ONES, b2, b3);
 #pragma unroll
-                for (int st = 0; st < STEPS; ++st) {
-                    const int step = p * STEPS + st;
-                    const unsigned char* words = here + w_at + ((step << 4) ^ w_swizzle);
-                    uint32_t w[4];
+                        for (int m = 0; m < 2; ++m) {
+                            const uint32_t lo = w[2 * m].v[st], hi = w[2 * m + 1].v[st];
+                            const uint32_t a0 = M::template pair<0>(lo), a1 = M::template pair<0>(hi);
+                            const uint32_t a2 = M::template pair<1>(lo), a3 = M::template pair<1>(hi);
+                            if (st == 0) M::template mma<true>(acc[m], a0, a1, a2, a3, b0, b1);
+                            else M::template mma<false>(acc[m], a0, a1, a2, a3, b0, b1);
+                            M::template mma<false>(acc[m], M::template pair<2>(lo), M::template pair<2>(hi), M::template pair<3>(lo),
+                                                   M::template pair<3>(hi), b2, b3);
+                        }
+                    }
+                    // C fragment: [0], [1] row g, columns 2c, 2c + 1; [2], [3] row g + 8.
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) w[h] = *reinterpret_cast<const uint32_t*>(words + 8 * h * (SLICE / 2));
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (g < cols) v = *reinterpret_cast<const uint4*>(here + x_at + step * 64);
-                    const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
-                    const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
-                    M::mma(ones, M::ONES, M::ONES, M::ONES, M::ONES, b0, b1);
-                    M::mma(ones, M::ONES, M::ONES, M::ONES, M::ONES, b2, b3);
+                    for (int h = 0; h < 4; ++h) {
+                        const float sc = M::to_f32(*reinterpret_cast<const uint16_t*>(sc_slice + h * 8 * 16 + p * 2));
+                        float zr = -M::BASE - 8.f;
+                        if (Z) zr = (8388608.f - M::BASE) - __uint_as_float(0x4B000000u | zr_slice[h * 8 * 8 + p]);   // 2^23 + z is exact
 #pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        const uint32_t lo = w[2 * m], hi = w[2 * m + 1];
-                        M::mma(acc[m], M::template pair<0>(lo), M::template pair<0>(hi), M::template pair<1>(lo), M::template pair<1>(hi), b0, b1);
-                        M::mma(acc[m], M::template pair<2>(lo), M::template pair<2>(hi), M::template pair<3>(lo), M::template pair<3>(hi), b2, b3);
+                        for (int i = 0; i < 2; ++i) {
+                            float& to = sum[h >> 1][2 * (h & 1) + i];
+                            to = fmaf(sc, fmaf(zr, ones[i], acc[h >> 1][2 * (h & 1) + i]), to);
+                        }
                     }
                 }
-                // C fragment: [0], [1] row g, columns 2c, 2c + 1; [2], [3] row g + 8.
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int h = 2 * m + (i >> 1);
-                        sum[m][i] = fmaf(sc[h][p], fmaf(zr[h][p], ones[i & 1], acc[m][i]), sum[m][i]);
-                    }
             }
         }
 
-        float* part = red + warp * layout.xrows * RED_PITCH;
+        // Two sets of sums: the next item's go to the other one, so one barrier per item is enough.
+        float* sums = red + (set * WARPS + team * a.split) * layout.red_floats;
+        set ^= 1;
+        float* part = sums + warp_k * layout.red_floats;
 #pragma unroll
         for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -359,22 +407,21 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
                 const int col = 2 * c + (i & 1);
                 if (col < cols) part[col * RED_PITCH + m * 16 + (i >> 1) * 8 + g] = sum[m][i];
             }
-        __syncthreads();
-        const int n_first = at.n0 - warp_row * ROWS;
-        for (int i = threadIdx.x; i < cols * tile_rows; i += THREADS) {
-            const int col = i / tile_rows, row = i - col * tile_rows;
-            if (n_first + row >= a.n) continue;
-            const float* p = red + ((row / ROWS) * a.split * layout.xrows + col) * RED_PITCH + row % ROWS;
+        team_sync(team, team_threads);
+        for (int i = warp_k * 32 + lane; i < cols * ROWS; i += team_threads) {
+            const int col = i / ROWS, row = i % ROWS;
+            if (at.n0 + row >= a.n) continue;
+            const float* p = sums + col * RED_PITCH + row;
             float v = 0.f;
-            for (int w = 0; w < a.split; ++w) v += p[w * layout.xrows * RED_PITCH];
-            static_cast<T*>(a.out)[static_cast<size_t>(at.r0 + col) * a.ldo + n_first + row] = M::from_f32(v);
+            for (int w = 0; w < a.split; ++w) v += p[w * layout.red_floats];
+            static_cast<T*>(a.out)[static_cast<size_t>(at.r0 + col) * a.ldo + at.n0 + row] = M::from_f32(v);
         }
-        __syncthreads();   // the next item's sums go to the same place
     }
+    cp_async_wait_all();
     if (timed_out && lane == 0) {
         // Unwind: let copies already in flight land before shared memory is released.
         for (int i = 0; i < stages && i < armed; ++i) {
-            const int behind = armed - 1 - i;   // the behind-th copy went to slot behind % stages, phase behind / stages
+            const int behind = armed - 1 - i;   // copy number `behind` went to slot behind % stages in phase behind / stages
             mbar_wait_bounded(&full[behind % stages], (behind / stages) & 1, never_flag, 2000000ull);
         }
     }
@@ -394,6 +441,29 @@ int w4_maps(CUtensorMap* map_w, CUtensorMap* map_x, const W4Args& a, const uint8
     return encode_tensor_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, x, xdims, xstrides, xbox, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Items of a call at most: every group may end in an item of its own.
+long long most_items(const W4Args& a) {
+    const long long tiles = (a.n + w4::ROWS - 1LL) / w4::ROWS;
+    if (!a.offsets) return tiles * ((a.rows + w4::COLS - 1) / w4::COLS);
+    return tiles * (a.rows / w4::COLS + (a.experts < a.rows ? a.experts : a.rows));
+}
+
+// Warps per team: the fewest rounds of (slices per warp + the item's own cost, about one slice) over all teams.
+int w4_split(const W4Args& a, int sms) {
+    const int slices = (a.k + w4::SLICE - 1) / w4::SLICE;
+    long long least = 0;
+    int best = 1;
+    for (int split = 1; split <= w4::WARPS && (split == 1 || split <= slices); split *= 2) {
+        const long long teams = static_cast<long long>(sms) * (w4::WARPS / split);
+        const long long cost = (most_items(a) + teams - 1) / teams * ((slices + split - 1) / split + 1);
+        if (least == 0 || cost < least) {
+            least = cost;
+            best = split;
+        }
+    }
+    return best;
+}
+
 template <typename T, int G, bool Z>
 int launch_w4(W4Args a, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
     auto kern = gemv_w4_kernel<T, G, Z>;
@@ -405,29 +475,20 @@ int launch_w4(W4Args a, const uint8_t* q, const void* x, long long ldx, cudaStre
         std::lock_guard<std::mutex> lk(mu);
         const bool cacheable = dev >= 0 && dev < 64;
         if (!cacheable || !sm_count[dev]) {
-            PRISM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448));
+            PRISM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, w4::SMEM_BYTES));
             PRISM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
             if (cacheable) sm_count[dev] = sms;
         } else {
             sms = sm_count[dev];
         }
     }
-    // Warps per 32 weight rows: as many as leave each four slices of k, more where the rows alone do not fill the SMs.
-    const int slices = (a.k + w4::SLICE - 1) / w4::SLICE;
-    const long long groups = a.offsets ? (a.experts < a.rows ? a.experts : a.rows) : 1;
-    auto most = [&](int split) {
-        const int tile_rows = w4::ROWS * (w4::WARPS / split);
-        return (a.n + tile_rows - 1LL) / tile_rows * (a.rows / w4::COLS + groups);
-    };
-    int split = 1;
-    while (split < w4::WARPS && slices >= 8 * split) split *= 2;
-    while (split < w4::WARPS && slices >= 2 * split && most(split) < sms) split *= 2;
-    a.split = split;
+    a.split = w4_split(a, sms);
     const w4::Layout layout(a.rows, a.experts);
     CUtensorMap map_w, map_x;
     if (int rc = w4_maps(&map_w, &map_x, a, q, x, ldx, layout.xrows)) return rc;
-    const int grid = static_cast<int>(most(split) < sms ? most(split) : sms);
-    kern<<<grid, w4::THREADS, layout.bytes, s>>>(a, map_w, map_x);
+    const int teams = w4::WARPS / a.split;
+    const long long blocks = (most_items(a) + teams - 1) / teams;
+    kern<<<static_cast<int>(blocks < sms ? blocks : sms), w4::THREADS, layout.bytes, s>>>(a, map_w, map_x);
     PRISM_CUDA_TRY(cudaGetLastError());
     count_launch();
     return PRISM_B200_OK;
@@ -472,8 +533,7 @@ extern "C" int prism_b200_gemv_w4(int dtype, int rows, int experts, int n, int k
         return set_error(PRISM_B200_ERR_MISALIGNED, "gemv_w4: x and q must be 16-byte aligned, x's row stride a multiple of 8");
     if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(out)) & 1u)
         return set_error(PRISM_B200_ERR_MISALIGNED, "gemv_w4: scales and out must be 2-byte aligned");
-    const int per = 128 / group;
-    const bool aligned = k % 128 == 0 && reinterpret_cast<uintptr_t>(scales) % (2 * per) == 0 && reinterpret_cast<uintptr_t>(zeros) % per == 0;
+    const bool aligned = k / group % w4::BLOCK == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0 && reinterpret_cast<uintptr_t>(zeros) % 8 == 0;
     if (int rc = bind_status_word()) return rc;
     const W4Args a{static_cast<const uint16_t*>(scales), zeros, offsets, out, ldo, rows, experts, n, k, 1, aligned ? 1 : 0};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
