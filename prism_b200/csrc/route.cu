@@ -10,6 +10,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace prism_b200 {
 namespace {
 
@@ -40,6 +42,141 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 }
 __device__ __forceinline__ float key_value(uint32_t key) {
     return __uint_as_float((key & 0x80000000u) ? (key ^ 0x80000000u) : ~key);
+}
+
+// The same for 16-bit types, from the bits: the order in the upper half, the lowest expert first among equals in the lower
+// half, so that all keys of a token differ and one maximum decides.
+template <typename T> __device__ __forceinline__ uint32_t packed_key(T v, int expert) {
+    const uint32_t b = *reinterpret_cast<const uint16_t*>(&v);
+    constexpr uint32_t INF = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+    if ((b & 0x7FFFu) > INF || b == (0x8000u | INF)) return 0u;
+    const uint32_t order = b == 0x8000u ? 0x8000u : (b & 0x8000u) ? (~b & 0xFFFFu) : (b | 0x8000u);
+    return (order << 16) | (0xFFFFu ^ static_cast<uint32_t>(expert));
+}
+template <typename T> __device__ __forceinline__ float packed_value(uint32_t key) {
+    const uint32_t order = key >> 16;
+    const uint16_t b = static_cast<uint16_t>((order & 0x8000u) ? (order ^ 0x8000u) : ~order);
+    return to_f32(*reinterpret_cast<const T*>(&b));
+}
+
+// The k choices of one token by one warp: lane j < k returns its choice's expert (-1: none) and logit, every lane the
+// largest logit and, with `all`, this lane's share of the sum of exp(logit - largest) over all experts.
+// A round takes the largest key of the lanes' best (redux.sync); the lane that has it goes on to its next.  Lanes with up
+// to four keys sort them first, so that this is a shift; others look through their keys again.
+template <typename T, int EPL>
+__device__ __forceinline__ void choose(const T* row, int experts, int k, bool all, int lane, int& id, float& logit, float& largest,
+                                       float& sum) {
+    constexpr bool SORTED = EPL <= 4;
+    uint32_t key[EPL];
+    int index[EPL];   // 32-bit types only
+    id = -1;
+    logit = largest = sum = 0.f;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            const int e = i * 32 + lane;
+            key[i] = e < experts ? packed_key(row[e], e) : 0u;
+        }
+        if constexpr (SORTED) {
+#pragma unroll
+            for (int n = EPL - 1; n > 0; --n)
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const uint32_t hi = max(key[i], key[i + 1]), lo = min(key[i], key[i + 1]);
+                    key[i] = hi;
+                    key[i + 1] = lo;
+                }
+        }
+        uint32_t best = key[0];
+#pragma unroll
+        for (int i = 1; i < EPL; ++i) best = max(best, key[i]);
+        uint32_t top = __reduce_max_sync(rt::FULL, best), mine = 0;
+        if (!top) return;
+        largest = packed_value<T>(top);
+        if (all) {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) sum += key[i] ? expf(packed_value<T>(key[i]) - largest) : 0.f;
+        }
+        for (int j = 0;; ) {
+            if (lane == j) mine = top;
+            if (++j == k) break;
+            if constexpr (SORTED) {
+                if (key[0] == top) {
+#pragma unroll
+                    for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1];
+                    key[EPL - 1] = 0;
+                }
+                best = key[0];
+            } else if (best == top) {
+                best = 0;
+#pragma unroll
+                for (int i = 0; i < EPL; ++i) best = max(best, key[i] < top ? key[i] : 0u);
+            }
+            top = __reduce_max_sync(rt::FULL, best);
+            if (!top) break;
+        }
+        if (mine) {
+            id = static_cast<int>(0xFFFFu ^ (mine & 0xFFFFu));
+            logit = packed_value<T>(mine);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+            const int e = i * 32 + lane;
+            key[i] = e < experts ? order_key(to_f32(row[e])) : 0u;
+            index[i] = e;
+        }
+        if constexpr (SORTED) {   // stable: a lane's experts ascend, equal keys stay in that order
+#pragma unroll
+            for (int n = EPL - 1; n > 0; --n)
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const bool swap = key[i + 1] > key[i];
+                    const uint32_t a = key[i], b = key[i + 1];
+                    const int x = index[i], y = index[i + 1];
+                    key[i] = swap ? b : a;
+                    key[i + 1] = swap ? a : b;
+                    index[i] = swap ? y : x;
+                    index[i + 1] = swap ? x : y;
+                }
+        }
+        uint32_t best = key[0];
+        int at = index[0];
+#pragma unroll
+        for (int i = 1; i < EPL; ++i)
+            if (key[i] > best) best = key[i], at = index[i];
+        uint32_t top = __reduce_max_sync(rt::FULL, best), mine = 0;
+        if (!top) return;
+        largest = key_value(top);
+        if (all) {
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) sum += key[i] ? expf(key_value(key[i]) - largest) : 0.f;
+        }
+        for (int j = 0;; ) {
+            const int win = __reduce_min_sync(rt::FULL, best == top ? at : 0x7fffffff);
+            if (lane == j) id = win, mine = top;
+            if (++j == k) break;
+            if ((win & 31) == lane) {
+                if constexpr (SORTED) {
+#pragma unroll
+                    for (int i = 0; i + 1 < EPL; ++i) key[i] = key[i + 1], index[i] = index[i + 1];
+                    key[EPL - 1] = 0;
+                    best = key[0];
+                    at = index[0];
+                } else {
+                    best = 0;
+#pragma unroll
+                    for (int i = 0; i < EPL; ++i) {
+                        if (i * 32 + lane == win) key[i] = 0;
+                        if (key[i] > best) best = key[i], at = i * 32 + lane;
+                    }
+                }
+            }
+            top = __reduce_max_sync(rt::FULL, best);
+            if (!top) break;
+        }
+        if (mine) logit = key_value(mine);
+    }
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -85,9 +222,7 @@ __device__ __forceinline__ int warp_exclusive_scan(const int* count, int* base, 
     return carry;
 }
 
-// One warp per token.  Lane l holds the keys of experts l, l + 32, ...; a round takes the largest key by one
-// redux.sync and the lowest expert that has it by another, so equal logits go to the lowest expert.  Then the block
-// ranks its choices: a token chooses an expert at most once, so a bit per (expert, token) says everything, and the rank
+// One warp per token (choose).  Then the block ranks its choices: a token chooses an expert at most once, so a bit per (expert, token) says everything, and the rank
 // of a choice is a popcount of the bits of earlier tokens.  With one block (grid 1, tokens <= CHUNK) the order is
 // complete here; otherwise the ranks are relative to the block and route_place_kernel adds the rest.
 template <typename T, int EPL>
@@ -113,41 +248,10 @@ __global__ void __launch_bounds__(1024, 1) route_choose_kernel(RouteArgs a) {
         for (int tt = warp; tt < n; tt += warps) {
             const size_t t = static_cast<size_t>(c0) + tt;
             const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-            uint32_t key[EPL];
-#pragma unroll
-            for (int i = 0; i < EPL; ++i) {
-                const int e = i * 32 + lane;
-                key[i] = e < a.experts ? order_key(to_f32(row[e])) : 0u;
-            }
-            uint32_t best = 0;
-            int best_i = 0;
-#pragma unroll
-            for (int i = 0; i < EPL; ++i)
-                if (key[i] > best) best = key[i], best_i = i;
-            uint32_t top = __reduce_max_sync(FULL, best);
-            const float largest = top ? key_value(top) : 0.f;
-            float sum = 0.f;
-            if (!a.renorm) {
-#pragma unroll
-                for (int i = 0; i < EPL; ++i) sum += key[i] ? expf(key_value(key[i]) - largest) : 0.f;
-            }
-            int id = -1;
-            float mine = 0.f;
-            for (int j = 0; j < k && top; ++j) {
-                const int win = __reduce_min_sync(FULL, best == top ? best_i * 32 + lane : 0x7fffffff);
-                if (lane == j) id = win, mine = expf(key_value(top) - largest);
-                if ((win & 31) == lane) {
-                    best = 0;
-#pragma unroll
-                    for (int i = 0; i < EPL; ++i) {
-                        if (i == best_i) key[i] = 0;
-                    }
-#pragma unroll
-                    for (int i = EPL - 1; i >= 0; --i)
-                        if (key[i] >= best && key[i]) best = key[i], best_i = i;
-                }
-                if (j + 1 < k) top = __reduce_max_sync(FULL, best);
-            }
+            int id;
+            float logit, largest, sum;
+            choose<T, EPL>(row, a.experts, k, !a.renorm, lane, id, logit, largest, sum);
+            const float mine = id >= 0 ? expf(logit - largest) : 0.f;
             sum = warp_sum(a.renorm ? mine : sum);
             if (lane < k) {
                 a.ids[t * k + lane] = id;
@@ -196,6 +300,8 @@ __global__ void __launch_bounds__(1024, 1) route_choose_kernel(RouteArgs a) {
         __syncthreads();
     }
     if (!single)
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (!single)
         for (int e = threadIdx.x; e < a.experts; e += blockDim.x)
             a.counts[static_cast<size_t>(blockIdx.x) * a.experts + e] = running[e];
 }
@@ -209,13 +315,18 @@ __global__ void __launch_bounds__(1024, 1) route_place_kernel(RouteArgs a) {
     __shared__ int all[EP], before[EP], base[EP];
     __shared__ int total;
     const int lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // launched while the first kernel still runs
+    const int first = blockIdx.x * a.tokens_per_block;
+    const int last = min(a.tokens, first + a.tokens_per_block);
+    const int begin = first * a.k + threadIdx.x, end = last * a.k;
+    int id = begin < end ? a.ids[begin] : -1, rank = begin < end ? a.pos[begin] : 0;   // before the counts: one latency for both
     for (int e = threadIdx.x; e < EP; e += blockDim.x) all[e] = before[e] = 0;
     __syncthreads();
     {
         const int e = threadIdx.x % EP, groups = blockDim.x / EP, blocks = gridDim.x;
         if (e < a.experts) {
             int sum = 0, pre = 0;
-#pragma unroll 8
+#pragma unroll 10
             for (int b = threadIdx.x / EP; b < blocks; b += groups) {
                 const int v = a.counts[static_cast<size_t>(b) * a.experts + e];
                 sum += v;
@@ -235,17 +346,15 @@ __global__ void __launch_bounds__(1024, 1) route_place_kernel(RouteArgs a) {
         if (lane == 0) total = sum;
     }
     __syncthreads();
-    const int first = blockIdx.x * a.tokens_per_block;
-    const int last = min(a.tokens, first + a.tokens_per_block);
-    const int end = last * a.k;
-    for (int i = first * a.k + threadIdx.x; i < end; i += blockDim.x) {
-        const int id = a.ids[i];
+    for (int i = begin; i < end;) {
         if (id >= 0) {
-            const int p = base[id] + before[id] + a.pos[i];
+            const int p = base[id] + before[id] + rank;
             a.pos[i] = p;
             a.order[p] = i;
         }
         if (i >= total) a.order[i] = -1;
+        i += blockDim.x;
+        if (i < end) id = a.ids[i], rank = a.pos[i];
     }
 }
 
@@ -284,14 +393,18 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const T* logits, long l
         top = warp_max(top);
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < EPL; ++i) sum += v[i] > -INFINITY ? expf(v[i] - top) : 0.f;
-        sum = warp_sum(sum);
+        for (int i = 0; i < EPL; ++i) {
+            v[i] = v[i] > -INFINITY ? expf(v[i] - top) : 0.f;
+            sum += v[i];
+        }
+        const float scale = 1.f / warp_sum(sum);
+        const bool some = top > -INFINITY;   // a row without an open expert has no gradient
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
             const int e = i * 32 + lane;
-            if (e < experts) row[e] = from_f32<T>(v[i] > -INFINITY ? expf(v[i] - top) / sum * -mean : 0.f);
+            if (e < experts) row[e] = from_f32<T>(v[i] != 0.f ? v[i] * scale * -mean : 0.f);
         }
-        p = id >= 0 ? expf(to_f32(in[id]) - top) / sum : 0.f;
+        p = id >= 0 && some ? expf(to_f32(in[id]) - top) * scale : 0.f;
     }
     __syncwarp();
     if (id >= 0) row[id] = from_f32<T>(p * (g - mean));
@@ -471,13 +584,22 @@ int launch_choose(const RouteArgs& a, int blocks, int threads, cudaStream_t s) {
 
 int launch_place(const RouteArgs& a, int blocks, cudaStream_t s) {
     const int per_lane = (a.experts + 31) / 32;
-    if (per_lane <= 1) route_place_kernel<1><<<blocks, 1024, 0, s>>>(a);
-    else if (per_lane <= 2) route_place_kernel<2><<<blocks, 1024, 0, s>>>(a);
-    else if (per_lane <= 4) route_place_kernel<4><<<blocks, 1024, 0, s>>>(a);
-    else if (per_lane <= 8) route_place_kernel<8><<<blocks, 1024, 0, s>>>(a);
-    else if (per_lane <= 16) route_place_kernel<16><<<blocks, 1024, 0, s>>>(a);
-    else route_place_kernel<32><<<blocks, 1024, 0, s>>>(a);
-    PRISM_CUDA_TRY(cudaGetLastError());
+    void (*kern)(RouteArgs) = per_lane <= 1    ? route_place_kernel<1>
+                              : per_lane <= 2  ? route_place_kernel<2>
+                              : per_lane <= 4  ? route_place_kernel<4>
+                              : per_lane <= 8  ? route_place_kernel<8>
+                              : per_lane <= 16 ? route_place_kernel<16>
+                                               : route_place_kernel<32>;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its launch overlaps the first kernel's end
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PRISM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a));
     count_launch();
     return PRISM_B200_OK;
 }
