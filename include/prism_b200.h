@@ -307,14 +307,14 @@ int prism_b200_gemm_bf16_fill_mode(int mode);
  * the device: the products read the group borders (`offsets`) there, and nothing is copied to the host.
  *
  * Row matrices are given by a pointer, a width and a row stride `ld` in elements (ld >= width); rows are contiguous
- * inside.  Outputs must not overlap inputs.  Every call is one launch (route_topk: two above 128 tokens), results
+ * inside.  Outputs must not overlap inputs.  Every call is one launch (route_topk: two above 64 tokens), results
  * repeat bit for bit, and calls on several streams at once need only outputs (and workspaces) of their own.
  */
 
 /* Element types of the entry points that take one. */
 enum { PRISM_B200_F32 = 0, PRISM_B200_BF16 = 1, PRISM_B200_F16 = 2 };
 
-/* Bytes of scratch for prism_b200_route_topk (0 up to 128 tokens); 4-byte aligned, its contents do not matter. */
+/* Bytes of scratch for prism_b200_route_topk (0 up to 64 tokens); 4-byte aligned, its contents do not matter. */
 int prism_b200_route_workspace_size(int tokens, int experts, int k, size_t* bytes);
 
 /*

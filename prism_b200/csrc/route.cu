@@ -20,6 +20,7 @@ constexpr int MAX_EXPERTS = 1024;
 constexpr int MAX_CHOICES = 32;    // lane j of a token's warp holds its choice j
 constexpr int CHUNK = 128;         // tokens whose choices a block ranks at a time
 constexpr int WORDS = CHUNK / 32;
+constexpr int ONE_BLOCK = 64;      // tokens up to which one block makes the whole order: 128 took 7.4 us, 5.2 in two launches
 constexpr int MAX_BLOCKS = 148;    // one block of 32 warps per SM
 constexpr unsigned FULL = 0xffffffffu;
 }  // namespace rt
@@ -59,14 +60,14 @@ template <typename T> __device__ __forceinline__ float packed_value(uint32_t key
     return to_f32(*reinterpret_cast<const T*>(&b));
 }
 
-// The k choices of one token by one warp: lane j < k returns its choice's expert (-1: none) and logit, every lane the
+// The k choices of one token by one warp (row: its logits of experts lane, lane + 32, ...): lane j < k returns its choice's expert (-1: none) and logit, every lane the
 // largest logit and, with `all`, this lane's share of the sum of exp(logit - largest) over all experts.
 // A round takes the largest key of the lanes' best (redux.sync); the lane that has it goes on to its next.  Lanes with up
-// to four keys sort them first, so that this is a shift; others look through their keys again.
+// to eight keys sort them first, so that this is a shift; others look through their keys again.
 template <typename T, int EPL>
-__device__ __forceinline__ void choose(const T* row, int experts, int k, bool all, int lane, int& id, float& logit, float& largest,
+__device__ __forceinline__ void choose(const T (&row)[EPL], int experts, int k, bool all, int lane, int& id, float& logit, float& largest,
                                        float& sum) {
-    constexpr bool SORTED = EPL <= 4;
+    constexpr bool SORTED = EPL <= 8;
     uint32_t key[EPL];
     int index[EPL];   // 32-bit types only
     id = -1;
@@ -75,7 +76,7 @@ __device__ __forceinline__ void choose(const T* row, int experts, int k, bool al
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
             const int e = i * 32 + lane;
-            key[i] = e < experts ? packed_key(row[e], e) : 0u;
+            key[i] = e < experts ? packed_key(row[i], e) : 0u;
         }
         if constexpr (SORTED) {
 #pragma unroll
@@ -123,7 +124,7 @@ __device__ __forceinline__ void choose(const T* row, int experts, int k, bool al
 #pragma unroll
         for (int i = 0; i < EPL; ++i) {
             const int e = i * 32 + lane;
-            key[i] = e < experts ? order_key(to_f32(row[e])) : 0u;
+            key[i] = e < experts ? order_key(to_f32(row[i])) : 0u;
             index[i] = e;
         }
         if constexpr (SORTED) {   // stable: a lane's experts ascend, equal keys stay in that order
@@ -223,7 +224,7 @@ __device__ __forceinline__ int warp_exclusive_scan(const int* count, int* base, 
 }
 
 // One warp per token (choose).  Then the block ranks its choices: a token chooses an expert at most once, so a bit per (expert, token) says everything, and the rank
-// of a choice is a popcount of the bits of earlier tokens.  With one block (grid 1, tokens <= CHUNK) the order is
+// of a choice is a popcount of the bits of earlier tokens.  With one block (grid 1, tokens <= ONE_BLOCK) the order is
 // complete here; otherwise the ranks are relative to the block and route_place_kernel adds the rest.
 template <typename T, int EPL>
 __global__ void __launch_bounds__(1024, 1) route_choose_kernel(RouteArgs a) {
@@ -245,9 +246,19 @@ __global__ void __launch_bounds__(1024, 1) route_choose_kernel(RouteArgs a) {
     __syncthreads();
     for (int c0 = first; c0 < last; c0 += CHUNK) {
         const int n = min(CHUNK, last - c0);
+        T row[EPL], next[EPL];   // the next token's logits are on their way while this one's choices are made
+        auto load = [&](int tt) {
+            const T* from = static_cast<const T*>(a.logits) + (static_cast<size_t>(c0) + tt) * a.ld;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i)
+                if (i * 32 + lane < a.experts) next[i] = from[i * 32 + lane];
+        };
+        if (warp < n) load(warp);
         for (int tt = warp; tt < n; tt += warps) {
             const size_t t = static_cast<size_t>(c0) + tt;
-            const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) row[i] = next[i];
+            if (tt + warps < n) load(tt + warps);
             int id;
             float logit, largest, sum;
             choose<T, EPL>(row, a.experts, k, !a.renorm, lane, id, logit, largest, sum);
@@ -419,32 +430,51 @@ struct alignas(sizeof(T) * V) Vec {
     T v[V];
 };
 
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { using type = uint4; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<4> { using type = unsigned; };
+template <> struct RawOf<2> { using type = unsigned short; };
+
+// Rows pass through once: loads and stores that leave the caches to others.
+template <typename W> __device__ __forceinline__ W load_once(const void* p) {
+    using Raw = typename RawOf<sizeof(W)>::type;
+    const Raw r = sizeof(W) < 8 ? *static_cast<const Raw*>(p) : __ldcs(static_cast<const Raw*>(p));   // small pieces share sectors
+    return *reinterpret_cast<const W*>(&r);
+}
+template <typename W> __device__ __forceinline__ void store_once(void* p, const W& v) {
+    using Raw = typename RawOf<sizeof(W)>::type;
+    __stcs(static_cast<Raw*>(p), *reinterpret_cast<const Raw*>(&v));
+}
+
 // out[pos[t, j]] = x[t]; U: raw unit of the copy.
 template <typename U>
-__global__ void __launch_bounds__(256) route_gather_kernel(const U* x, long long ldx, int tokens, int k, int units, const int* pos,
-                                                           long long rows, U* out, long long ldo) {
+__global__ void __launch_bounds__(256) route_gather_kernel(const U* __restrict__ x, long long ldx, int tokens, int k, int units,
+                                                           const int* __restrict__ pos, long long rows, U* __restrict__ out,
+                                                           long long ldo) {
     const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     if (t >= static_cast<size_t>(tokens)) return;
     const U* src = x + t * ldx;
     const int* p = pos + t * k;
     for (int c = blockIdx.y * blockDim.x * 2 + threadIdx.x; c < units; c += gridDim.y * blockDim.x * 2) {
         const int c2 = c + blockDim.x;
-        const U v = src[c];
-        const U v2 = c2 < units ? src[c2] : v;
+        const U v = __ldcs(src + c);
+        const U v2 = c2 < units ? __ldcs(src + c2) : v;
         for (int j = 0; j < k; ++j) {
             const int r = p[j];
             if (r < 0 || r >= rows) continue;
             U* dst = out + static_cast<size_t>(r) * ldo;
-            dst[c] = v;
-            if (c2 < units) dst[c2] = v2;
+            __stcs(dst + c, v);
+            if (c2 < units) __stcs(dst + c2, v2);
         }
     }
 }
 
-// out[t] = sum over j of w[t, j] * y[pos[t, j]], added up in fp32 in the order of j and rounded once.
-template <typename T, int V>
-__global__ void __launch_bounds__(256) route_combine_kernel(const T* y, long long ldy, long long rows, int tokens, int k, int units,
-                                                            const int* pos, const float* weights, T* out, long long ldo) {
+// out[t] = sum over j of w[t, j] * y[pos[t, j]], added up in fp32 in the order of j and rounded once.  KB rows in flight.
+template <typename T, int V, int KB>
+__global__ void __launch_bounds__(256, 4) route_combine_kernel(const T* __restrict__ y, long long ldy, long long rows, int tokens, int k,
+                                                               int units, const int* __restrict__ pos,
+                                                               const float* __restrict__ weights, T* __restrict__ out, long long ldo) {
     using W = Vec<T, V>;
     const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     if (t >= static_cast<size_t>(tokens)) return;
@@ -454,18 +484,20 @@ __global__ void __launch_bounds__(256) route_combine_kernel(const T* y, long lon
         float acc[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = 0.f;
-        for (int j0 = 0; j0 < k; j0 += 4) {   // four rows in flight
-            W v[4];
-            bool live[4];
+        for (int j0 = 0; j0 < k; j0 += KB) {
+            int r[KB];
+            W v[KB];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int r = j0 + u < k ? p[j0 + u] : -1;
-                live[u] = r >= 0 && r < rows;
-                if (live[u]) v[u] = *reinterpret_cast<const W*>(y + static_cast<size_t>(r) * ldy + static_cast<size_t>(c) * V);
+            for (int u = 0; u < KB; ++u) {
+                r[u] = j0 + u < k ? p[j0 + u] : -1;
+                if (r[u] >= rows) r[u] = -1;
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (!live[u]) continue;
+            for (int u = 0; u < KB; ++u)
+                if (r[u] >= 0) v[u] = load_once<W>(y + static_cast<size_t>(r[u]) * ldy + static_cast<size_t>(c) * V);
+#pragma unroll
+            for (int u = 0; u < KB; ++u) {
+                if (r[u] < 0) continue;
                 const float w = wt ? wt[j0 + u] : 1.f;
 #pragma unroll
                 for (int i = 0; i < V; ++i) acc[i] = fmaf(w, to_f32(v[u].v[i]), acc[i]);
@@ -474,17 +506,19 @@ __global__ void __launch_bounds__(256) route_combine_kernel(const T* y, long lon
         W o;
 #pragma unroll
         for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(acc[i]);
-        *reinterpret_cast<W*>(out + t * ldo + static_cast<size_t>(c) * V) = o;
+        store_once(out + t * ldo + static_cast<size_t>(c) * V, o);
     }
 }
 
-// dy[pos[t, j]] = w[t, j] * dout[t] and dw[t, j] = dot(dout[t], y[pos[t, j]]): one pass over the rows, the dot products
-// in fp32 in registers (KT of them), added up over the token's threads by shuffles and then in warp order.
+// dy[pos[t, j]] = w[t, j] * dout[t] and dw[t, j] = dot(dout[t], y[pos[t, j]]): one pass over the rows, KB of them in flight;
+// the dot products (KT of them) in fp32 in registers, added up over the token's threads by shuffles and then in warp order.
 template <typename T, int V, int KT>
-__global__ void __launch_bounds__(256) route_combine_grad_kernel(const T* dout, long long ldd, const T* y, long long ldy,
-                                                                 long long rows, int tokens, int k, int units, const int* pos,
-                                                                 const float* weights, T* dy, long long lddy, float* dw) {
+__global__ void __launch_bounds__(256) route_combine_grad_kernel(const T* __restrict__ dout, long long ldd, const T* __restrict__ y,
+                                                                 long long ldy, long long rows, int tokens, int k, int units,
+                                                                 const int* __restrict__ pos, const float* __restrict__ weights,
+                                                                 T* __restrict__ dy, long long lddy, float* __restrict__ dw) {
     using W = Vec<T, V>;
+    constexpr int KB = KT < 8 ? KT : 8;
     __shared__ float part[8][KT];
     const size_t t = static_cast<size_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const bool here = t < static_cast<size_t>(tokens);   // blockDim.x is a multiple of 32: whole warps
@@ -503,21 +537,27 @@ __global__ void __launch_bounds__(256) route_combine_grad_kernel(const T* dout, 
             w[j] = r[j] >= 0 ? weights[t * k + j] : 0.f;
         }
         for (int c = threadIdx.x; c < units; c += blockDim.x) {
-            const W d = *reinterpret_cast<const W*>(dout + t * ldd + static_cast<size_t>(c) * V);
-            float df[V];
+            const size_t at = static_cast<size_t>(c) * V;
+            const W d = load_once<W>(dout + t * ldd + at);
 #pragma unroll
-            for (int i = 0; i < V; ++i) df[i] = to_f32(d.v[i]);
+            for (int j0 = 0; j0 < KT; j0 += KB) {
+                W a[KB];
 #pragma unroll
-            for (int j = 0; j < KT; ++j) {
-                if (r[j] < 0) continue;
-                const W a = *reinterpret_cast<const W*>(y + static_cast<size_t>(r[j]) * ldy + static_cast<size_t>(c) * V);
-                W o;
+                for (int u = 0; u < KB; ++u)
+                    if (r[j0 + u] >= 0) a[u] = load_once<W>(y + static_cast<size_t>(r[j0 + u]) * ldy + at);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    acc[j] = fmaf(df[i], to_f32(a.v[i]), acc[j]);
-                    o.v[i] = from_f32<T>(w[j] * df[i]);
+                for (int u = 0; u < KB; ++u) {
+                    const int j = j0 + u;
+                    if (r[j] < 0) continue;
+                    W o;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float df = to_f32(d.v[i]);
+                        acc[j] = fmaf(df, to_f32(a[u].v[i]), acc[j]);
+                        o.v[i] = from_f32<T>(w[j] * df);
+                    }
+                    store_once(dy + static_cast<size_t>(r[j]) * lddy + at, o);
                 }
-                *reinterpret_cast<W*>(dy + static_cast<size_t>(r[j]) * lddy + static_cast<size_t>(c) * V) = o;
             }
         }
     }
@@ -536,7 +576,7 @@ __global__ void __launch_bounds__(256) route_combine_grad_kernel(const T* dout, 
 }
 
 int blocks_for(int tokens) {
-    if (tokens <= rt::CHUNK) return 1;
+    if (tokens <= rt::ONE_BLOCK) return 1;
     const int by_warp = (tokens + 31) / 32;   // a token per warp while that leaves SMs without a block
     return by_warp < rt::MAX_BLOCKS ? by_warp : rt::MAX_BLOCKS;
 }
@@ -611,10 +651,13 @@ int launch_grad(const void* logits, long long ld, int tokens, int experts, int k
     const int per_lane = (experts + 31) / 32;
     const T* l = static_cast<const T*>(logits);
     T* o = static_cast<T*>(out);
-    if (renorm || per_lane <= 1) route_grad_kernel<T, 1><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
-    else if (per_lane <= 4) route_grad_kernel<T, 4><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
-    else if (per_lane <= 8) route_grad_kernel<T, 8><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
-    else route_grad_kernel<T, 32><<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
+    auto kern = renorm || per_lane <= 1 ? route_grad_kernel<T, 1>
+                : per_lane <= 2         ? route_grad_kernel<T, 2>
+                : per_lane <= 4         ? route_grad_kernel<T, 4>
+                : per_lane <= 8         ? route_grad_kernel<T, 8>
+                : per_lane <= 16        ? route_grad_kernel<T, 16>
+                                        : route_grad_kernel<T, 32>;
+    kern<<<blocks, 256, 0, s>>>(l, ld, tokens, experts, k, renorm, ids, weights, dweights, o);
     PRISM_CUDA_TRY(cudaGetLastError());
     count_launch();
     return PRISM_B200_OK;
@@ -646,8 +689,8 @@ int launch_combine(const void* y, long long ldy, long long rows, int tokens, int
     const dim3 block = row_block(units, 16);
     const int pieces = (units + 255) / 256;
     const dim3 grid((tokens + block.y - 1) / block.y, pieces < 64 ? pieces : 64);
-    route_combine_kernel<T, V><<<grid, block, 0, s>>>(static_cast<const T*>(y), ldy, rows, tokens, k, units, pos, weights,
-                                                      static_cast<T*>(out), ldo);
+    auto kern = k <= 2 ? route_combine_kernel<T, V, 2> : k <= 4 ? route_combine_kernel<T, V, 4> : route_combine_kernel<T, V, 8>;
+    kern<<<grid, block, 0, s>>>(static_cast<const T*>(y), ldy, rows, tokens, k, units, pos, weights, static_cast<T*>(out), ldo);
     PRISM_CUDA_TRY(cudaGetLastError());
     count_launch();
     return PRISM_B200_OK;

@@ -101,7 +101,7 @@ def _run(device, fn, *args) -> None:
 # ---------------------------------------------------------------------------
 @functools.lru_cache(maxsize=256)
 def route_workspace_size(tokens: int, experts: int, k: int) -> int:
-    """Bytes of scratch that route_topk needs (0 up to 128 tokens)."""
+    """Bytes of scratch that route_topk needs (0 up to 64 tokens)."""
     out = ctypes.c_size_t(0)
     _lib.check(load().prism_b200_route_workspace_size(int(tokens), int(experts), int(k), ctypes.byref(out)))
     return int(out.value)

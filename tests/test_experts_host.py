@@ -24,8 +24,8 @@ def lib():
 
 def test_route_workspace(lib):
     size = lambda t, e, k: pb.route_workspace_size(t, e, k)  # noqa: E731
-    assert size(0, 8, 2) == size(1, 1024, 32) == size(128, 64, 8) == 0
-    assert size(129, 64, 8) == 5 * 64 * 4
+    assert size(0, 8, 2) == size(1, 1024, 32) == size(64, 64, 8) == 0
+    assert size(65, 64, 8) == 3 * 64 * 4
     assert size(1 << 20, 64, 8) == 148 * 64 * 4
     for bad in ((-1, 8, 2), (1, 0, 1), (1, 1025, 2), (1, 8, 9), (1, 64, 33), (1 << 29, 64, 4)):
         with pytest.raises(pb.PrismB200Error):

@@ -52,7 +52,7 @@ def make_logits(T, E, dtype, seed, masked=0.0):
     return l.to(dtype)
 
 
-@pytest.mark.parametrize("T", [1, 3, 32, 127, 128, 129, 500, 4736, 4737, 20001])
+@pytest.mark.parametrize("T", [1, 3, 32, 63, 64, 65, 127, 129, 500, 4736, 4737, 20001])
 @pytest.mark.parametrize("E,k", [(8, 2), (64, 8)])
 def test_token_counts(pb, T, E, k):
     check_route(pb, make_logits(T, E, torch.float32, T + E, 0.1), k, True)
