@@ -439,12 +439,13 @@ template <> struct RawOf<2> { using type = unsigned short; };
 // Rows pass through once: loads and stores that leave the caches to others.
 template <typename W> __device__ __forceinline__ W load_once(const void* p) {
     using Raw = typename RawOf<sizeof(W)>::type;
-    const Raw r = sizeof(W) < 8 ? *static_cast<const Raw*>(p) : __ldcs(static_cast<const Raw*>(p));   // small pieces share sectors
+    const Raw r = sizeof(W) < 8 ? __ldca(static_cast<const Raw*>(p)) : __ldcs(static_cast<const Raw*>(p));   // small pieces share sectors
     return *reinterpret_cast<const W*>(&r);
 }
 template <typename W> __device__ __forceinline__ void store_once(void* p, const W& v) {
     using Raw = typename RawOf<sizeof(W)>::type;
-    __stcs(static_cast<Raw*>(p), *reinterpret_cast<const Raw*>(&v));
+    if (sizeof(W) < 8) *static_cast<Raw*>(p) = *reinterpret_cast<const Raw*>(&v);
+    else __stcs(static_cast<Raw*>(p), *reinterpret_cast<const Raw*>(&v));
 }
 
 // out[pos[t, j]] = x[t]; U: raw unit of the copy.
@@ -480,13 +481,17 @@ __global__ void __launch_bounds__(256, 4) route_combine_kernel(const T* __restri
     if (t >= static_cast<size_t>(tokens)) return;
     const int* p = pos + t * k;
     const float* wt = weights ? weights + t * k : nullptr;
-    for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < units; c += gridDim.y * blockDim.x) {
-        float acc[V];
+    constexpr int U = V >= 4 ? 1 : 4;   // vectors of a row per thread: narrow ones share the reading of positions and weights
+    const int step = blockDim.x;
+    for (int c = blockIdx.y * step * U + threadIdx.x; c < units; c += gridDim.y * step * U) {
+        float acc[U][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+        for (int n = 0; n < U; ++n)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[n][i] = 0.f;
         for (int j0 = 0; j0 < k; j0 += KB) {
             int r[KB];
-            W v[KB];
+            W v[KB][U];
 #pragma unroll
             for (int u = 0; u < KB; ++u) {
                 r[u] = j0 + u < k ? p[j0 + u] : -1;
@@ -494,19 +499,28 @@ __global__ void __launch_bounds__(256, 4) route_combine_kernel(const T* __restri
             }
 #pragma unroll
             for (int u = 0; u < KB; ++u)
-                if (r[u] >= 0) v[u] = load_once<W>(y + static_cast<size_t>(r[u]) * ldy + static_cast<size_t>(c) * V);
+#pragma unroll
+                for (int n = 0; n < U; ++n)
+                    if (r[u] >= 0 && c + n * step < units)
+                        v[u][n] = load_once<W>(y + static_cast<size_t>(r[u]) * ldy + static_cast<size_t>(c + n * step) * V);
 #pragma unroll
             for (int u = 0; u < KB; ++u) {
                 if (r[u] < 0) continue;
                 const float w = wt ? wt[j0 + u] : 1.f;
 #pragma unroll
-                for (int i = 0; i < V; ++i) acc[i] = fmaf(w, to_f32(v[u].v[i]), acc[i]);
+                for (int n = 0; n < U; ++n)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) acc[n][i] = fmaf(w, to_f32(v[u][n].v[i]), acc[n][i]);
             }
         }
-        W o;
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(acc[i]);
-        store_once(out + t * ldo + static_cast<size_t>(c) * V, o);
+        for (int n = 0; n < U; ++n) {
+            if (c + n * step >= units) break;
+            W o;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = from_f32<T>(acc[n][i]);
+            store_once(out + t * ldo + static_cast<size_t>(c + n * step) * V, o);
+        }
     }
 }
 
@@ -687,7 +701,8 @@ int launch_combine(const void* y, long long ldy, long long rows, int tokens, int
                    void* out, long long ldo, cudaStream_t s) {
     const int units = width / V;
     const dim3 block = row_block(units, 16);
-    const int pieces = (units + 255) / 256;
+    const int per_block = V >= 4 ? 256 : 1024;
+    const int pieces = (units + per_block - 1) / per_block;
     const dim3 grid((tokens + block.y - 1) / block.y, pieces < 64 ? pieces : 64);
     auto kern = k <= 2 ? route_combine_kernel<T, V, 2> : k <= 4 ? route_combine_kernel<T, V, 4> : route_combine_kernel<T, V, 8>;
     kern<<<grid, block, 0, s>>>(static_cast<const T*>(y), ldy, rows, tokens, k, units, pos, weights, static_cast<T*>(out), ldo);
