@@ -382,8 +382,7 @@ int prism_b200_grouped_gemm_bf16_wgrad(int experts, int rows, int n, int k, cons
  *   scales  [experts][n][k / group]
  *   zeros   [experts][n][k / group]  one byte each, or NULL: 8 everywhere
  *   offsets [experts + 1]            the rows of each expert's matrix, as above; NULL: one matrix (experts = 1) for all rows
- * group 32, 64 or 128, k a multiple of it; any n.  x and q 16-byte aligned, ldx a multiple of 8.  A row of x that holds
- * an infinity or NaN gives outputs that are not finite (possibly NaN where the sum would be an infinity).
+ * group 32, 64 or 128, k a multiple of it; any n; zeros 0 .. 15.  x and q 16-byte aligned, ldx a multiple of 8.
  */
 int prism_b200_gemv_w4(int dtype, int rows, int experts, int n, int k, int group, const void* x, long long ldx, const uint8_t* q,
                        const void* scales, const uint8_t* zeros, const int* offsets, void* out, long long ldo, void* stream);

@@ -7,10 +7,9 @@
 // 23 bytes (46 weights) per clock to keep up with HBM.
 //   * Products and sums are mma.sync m16n8k16 with fp32 accumulators: 16 weight rows x 16 k against up to 8 rows of x.
 //     tcgen05 would want the converted weights in shared memory, a round trip of four times the bytes read here.
-//   * A nibble becomes an operand by one shift and one LOP3: put into the mantissa of 16.0 (bf16) or 64.0 (fp16) it makes
-//     16 + q or 64 + q, exactly.  The base and z are taken off afterwards, once per group, in fp32:
-//     sum (q - z) x = sum (16 + q) x - (16 + z) * sum x, with sum x from one more MMA whose weight operand is all ones.
-//     The larger terms cost 3 or 5 bits of the fp32 accumulator's 24, far below the rounding of y to 16 bits.
+//   * A nibble becomes an operand by one shift and one LOP3, which put it into the mantissa of 16.0 (bf16) or 64.0 (fp16),
+//     and one packed subtraction of 16 + z: q - z, exactly.  So the products are exact and only the sums round, in fp32.
+//     (Taking the base and z off afterwards, with sum x from one more MMA, took the same time and costs bits.)
 //   * A 32-bit word holds 8 consecutive k; the MMA's order of k is free as long as both operands follow it, so the
 //     pairs are (k, k + 4) as the masks deliver them, and x is brought into that order by four PRMTs per 8 values.
 //   * The four lanes of a quad take one, two or four consecutive words each, 32, 64 or 128 k together: a group, whose sum is
@@ -21,7 +20,8 @@
 //     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
 //     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
 //   * The team's sums meet in shared memory once per item, added in warp order.
-// Integer instructions (ALU pipe, half rate) are the next bound: 7 per word of 8 weights in bf16, 5 in fp16.
+// What bounds it now: at 16384 x 16384 and one row 39 us, where the copies alone take 25 and the arithmetic alone 31 (shifts
+// and masks on the half-rate ALU pipe and mma.sync at 16 cycles per instruction and scheduler take about 22 each).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -42,7 +42,7 @@ constexpr int W_BYTES = ROWS * SLICE / 2;
 constexpr int RED_PITCH = ROWS + 4;      // a fragment's 8 x 4 places lie in 32 banks
 constexpr int BLOCK = 8;                 // groups whose scales are copied at a time
 constexpr int SC_BYTES = ROWS * BLOCK * 3;   // a block: 16 bytes of scales per row, then 8 bytes of zero points per row
-constexpr int MAX_STAGES = 6;
+constexpr int MAX_STAGES = 3;            // more only crowd the memory: copies alone of 16384 x 16384 take 25 us with three, 37 with six
 constexpr int MAX_EXPERTS = 1024;
 constexpr int SMEM_BYTES = 232448;
 
@@ -73,8 +73,13 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
 
 template <typename T> struct W4Type;
 template <> struct W4Type<__nv_bfloat16> {
-    static constexpr uint32_t ONES = 0x3F803F80u;
-    static constexpr float BASE = 16.f;
+    static constexpr uint32_t EIGHT = 0x41C041C0u;   // 16 + 8, twice
+    // 16 + z, twice
+    static __device__ __forceinline__ uint32_t zero(uint32_t z) { return (z << 3) * 0x10001u | 0x41804180u; }
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
     // nibble i of the word's two halves -> (16 + q) twice: 16.0 is 0x4180, the mantissa's top four bits are bits 3-6
     template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
         const uint32_t s = I == 0 ? w * 8u : w >> (4 * I - 3);
@@ -97,8 +102,12 @@ template <> struct W4Type<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct W4Type<__half> {
-    static constexpr uint32_t ONES = 0x3C003C00u;
-    static constexpr float BASE = 64.f;
+    static constexpr uint32_t EIGHT = 0x54805480u;   // 64 + 8, twice
+    static __device__ __forceinline__ uint32_t zero(uint32_t z) { return (z << 4) * 0x10001u | 0x54005400u; }   // 64 + z, twice
+    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
+        const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
     // (64 + q) twice: 64.0 is 0x5400, and a nibble on bits 4-7 of its ten-bit mantissa counts in ones; left shifts are
     // multiplications (FMA pipe), so a word takes one shift and four LOP3
     template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
@@ -319,7 +328,7 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
     bool timed_out = false;
     // Where a lane reads in a stage: its words of row g (rows 8 apart have the same swizzle), its pieces of x.
     const int w_row = g * (SLICE / 2), w_swizzle = (g >> 1) & 3;
-    const int x_row = W_BYTES + g * X_PITCH;
+    const int x_row = W_BYTES + min(g, layout.xrows - 1) * X_PITCH;   // columns without a row of x repeat one; they are not stored
     for (at.t = t_first; at.t < total; at.t += t_step) {
         at.decode(a, first, last, items);
         const int cols = at.cols;
@@ -359,37 +368,35 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
                     const unsigned char* words = here + w_row + ((((byte >> 4) ^ w_swizzle) << 4) | (byte & 15));
 #pragma unroll
                     for (int h = 0; h < 4; ++h) w[h] = *reinterpret_cast<const Words*>(words + 8 * h * (SLICE / 2));
-                    float acc[2][4], ones[4];
+                    float acc[2][4];
+                    uint32_t zr[4];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) zr[h] = Z ? M::zero(zr_slice[h * 8 * 8 + p]) : M::EIGHT;
 #pragma unroll
                     for (int st = 0; st < STEPS; ++st) {
-                        uint4 v = make_uint4(0, 0, 0, 0);
-                        if (g < cols) v = *reinterpret_cast<const uint4*>(here + x_row + (p * G + (c * STEPS + st) * 8) * 2);
+                        const uint4 v = *reinterpret_cast<const uint4*>(here + x_row + (p * G + (c * STEPS + st) * 8) * 2);
                         const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
                         const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
-                        if (st == 0) M::template mma<true>(ones, M::ONES, M::ONES, M::ONES, M::ONES, b0, b1);
-                        else M::template mma<false>(ones, M::ONES, M::ONES, M::ONES, M::ONES, b0, b1);
-                        M::template mma<false>(ones, M::ONES, M::ONES, M::ONES, M::ONES, b2, b3);
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             const uint32_t lo = w[2 * m].v[st], hi = w[2 * m + 1].v[st];
-                            const uint32_t a0 = M::template pair<0>(lo), a1 = M::template pair<0>(hi);
-                            const uint32_t a2 = M::template pair<1>(lo), a3 = M::template pair<1>(hi);
+                            const uint32_t zl = zr[2 * m], zh = zr[2 * m + 1];
+                            const uint32_t a0 = M::sub(M::template pair<0>(lo), zl), a1 = M::sub(M::template pair<0>(hi), zh);
+                            const uint32_t a2 = M::sub(M::template pair<1>(lo), zl), a3 = M::sub(M::template pair<1>(hi), zh);
                             if (st == 0) M::template mma<true>(acc[m], a0, a1, a2, a3, b0, b1);
                             else M::template mma<false>(acc[m], a0, a1, a2, a3, b0, b1);
-                            M::template mma<false>(acc[m], M::template pair<2>(lo), M::template pair<2>(hi), M::template pair<3>(lo),
-                                                   M::template pair<3>(hi), b2, b3);
+                            M::template mma<false>(acc[m], M::sub(M::template pair<2>(lo), zl), M::sub(M::template pair<2>(hi), zh),
+                                                   M::sub(M::template pair<3>(lo), zl), M::sub(M::template pair<3>(hi), zh), b2, b3);
                         }
                     }
                     // C fragment: [0], [1] row g, columns 2c, 2c + 1; [2], [3] row g + 8.
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         const float sc = M::to_f32(*reinterpret_cast<const uint16_t*>(sc_slice + h * 8 * 16 + p * 2));
-                        float zr = -M::BASE - 8.f;
-                        if (Z) zr = (8388608.f - M::BASE) - __uint_as_float(0x4B000000u | zr_slice[h * 8 * 8 + p]);   // 2^23 + z is exact
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             float& to = sum[h >> 1][2 * (h & 1) + i];
-                            to = fmaf(sc, fmaf(zr, ones[i], acc[h >> 1][2 * (h & 1) + i]), to);
+                            to = fmaf(sc, acc[h >> 1][2 * (h & 1) + i], to);
                         }
                     }
                 }
@@ -533,6 +540,8 @@ extern "C" int prism_b200_gemv_w4(int dtype, int rows, int experts, int n, int k
         return set_error(PRISM_B200_ERR_MISALIGNED, "gemv_w4: x and q must be 16-byte aligned, x's row stride a multiple of 8");
     if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(out)) & 1u)
         return set_error(PRISM_B200_ERR_MISALIGNED, "gemv_w4: scales and out must be 2-byte aligned");
+    if (rows_overlap(out, rows, n, ldo, x, rows, k, ldx, 2))
+        return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "gemv_w4: out overlaps x");
     const bool aligned = k / group % w4::BLOCK == 0 && reinterpret_cast<uintptr_t>(scales) % 16 == 0 && reinterpret_cast<uintptr_t>(zeros) % 8 == 0;
     if (int rc = bind_status_word()) return rc;
     const W4Args a{static_cast<const uint16_t*>(scales), zeros, offsets, out, ldo, rows, experts, n, k, 1, aligned ? 1 : 0};

@@ -157,7 +157,7 @@ def route_topk_grad(logits: torch.Tensor, ids: torch.Tensor, weights: torch.Tens
     _tensor("weights", weights, device, torch.float32, (tokens, k))
     _tensor("dweights", dweights, device, torch.float32, (tokens, k))
     if out is None:
-        out = torch.empty((tokens, experts), dtype=logits.dtype, device=device)
+        out = logits.new_empty((tokens, experts))
     else:
         _tensor("out", out, device, logits.dtype, (tokens, experts))
     _run(device, load().prism_b200_route_topk_grad, tokens, experts, k, code, logits.data_ptr(), ld, int(bool(renormalize)),
@@ -180,8 +180,9 @@ def route_gather(x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor | None = 
     tokens, width = x.shape
     _, k = _pos(pos, x.device, tokens)
     if out is None:
-        out = torch.empty((tokens * k, width), dtype=x.dtype, device=x.device)
-    ldo = _rows("out", out, x.device, x.dtype, None, width)
+        out, ldo = x.new_empty((tokens * k, width)), width
+    else:
+        ldo = _rows("out", out, x.device, x.dtype, None, width)
     _run(x.device, load().prism_b200_route_gather, _code("x", x.dtype), tokens, k, width, x.data_ptr(), ldx, pos.data_ptr(),
          out.shape[0], out.data_ptr(), ldo)
     return out
@@ -197,8 +198,9 @@ def route_combine(y: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor | No
     if weights is not None:
         _tensor("weights", weights, y.device, torch.float32, (tokens, k))
     if out is None:
-        out = torch.empty((tokens, width), dtype=y.dtype, device=y.device)
-    ldo = _rows("out", out, y.device, y.dtype, tokens, width)
+        out, ldo = y.new_empty((tokens, width)), width
+    else:
+        ldo = _rows("out", out, y.device, y.dtype, tokens, width)
     _run(y.device, load().prism_b200_route_combine, _code("y", y.dtype), tokens, k, width, y.data_ptr(), ldy, rows, pos.data_ptr(),
          None if weights is None else weights.data_ptr(), out.data_ptr(), ldo)
     return out
@@ -214,10 +216,11 @@ def route_combine_grad(dout: torch.Tensor, y: torch.Tensor, pos: torch.Tensor, w
     _tensor("weights", weights, dout.device, torch.float32, (tokens, k))
     rows = y.shape[0]
     if dy is None:
-        dy = torch.empty((rows, width), dtype=y.dtype, device=y.device)
-    lddy = _rows("dy", dy, dout.device, dout.dtype, rows, width)
+        dy, lddy = y.new_empty((rows, width)), width
+    else:
+        lddy = _rows("dy", dy, dout.device, dout.dtype, rows, width)
     if dweights is None:
-        dweights = torch.empty((tokens, k), dtype=torch.float32, device=dout.device)
+        dweights = weights.new_empty((tokens, k))
     else:
         _tensor("dweights", dweights, dout.device, torch.float32, (tokens, k))
     _run(dout.device, load().prism_b200_route_combine_grad, _code("dout", dout.dtype), tokens, k, width, dout.data_ptr(), ldd,
@@ -245,8 +248,9 @@ def grouped_gemm_bf16(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, o
         raise ValueError(f"k mismatch: x {tuple(x.shape)}, w {tuple(w.shape)}")
     _tensor("offsets", offsets, x.device, torch.int32, (experts + 1,))
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.bfloat16, device=x.device)
-    ldo = _rows("out", out, x.device, torch.bfloat16, rows, n)
+        out, ldo = x.new_empty((rows, n)), n
+    else:
+        ldo = _rows("out", out, x.device, torch.bfloat16, rows, n)
     _run(x.device, load().prism_b200_grouped_gemm_bf16, experts, rows, n, k, x.data_ptr(), ldx, w.data_ptr(), offsets.data_ptr(),
          out.data_ptr(), ldo)
     return out
@@ -261,8 +265,9 @@ def grouped_gemm_bf16_dgrad(dy: torch.Tensor, w: torch.Tensor, offsets: torch.Te
         raise ValueError(f"n mismatch: dy {tuple(dy.shape)}, w {tuple(w.shape)}")
     _tensor("offsets", offsets, dy.device, torch.int32, (experts + 1,))
     if out is None:
-        out = torch.empty((rows, k), dtype=torch.bfloat16, device=dy.device)
-    ldo = _rows("out", out, dy.device, torch.bfloat16, rows, k)
+        out, ldo = dy.new_empty((rows, k)), k
+    else:
+        ldo = _rows("out", out, dy.device, torch.bfloat16, rows, k)
     _run(dy.device, load().prism_b200_grouped_gemm_bf16_dgrad, experts, rows, n, k, dy.data_ptr(), lddy, w.data_ptr(),
          offsets.data_ptr(), out.data_ptr(), ldo)
     return out
@@ -327,8 +332,9 @@ def gemv_w4(x: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: torch
     if offsets is not None:
         _tensor("offsets", offsets, device, torch.int32, (experts + 1,))
     if out is None:
-        out = torch.empty((rows, n), dtype=x.dtype, device=device)
-    ldo = _rows("out", out, device, x.dtype, rows, n)
+        out, ldo = x.new_empty((rows, n)), n
+    else:
+        ldo = _rows("out", out, device, x.dtype, rows, n)
     _run(device, load().prism_b200_gemv_w4, _CODES[x.dtype], rows, experts, n, k, k // groups, x.data_ptr(), ldx, q.data_ptr(),
          scales.data_ptr(), None if zeros is None else zeros.data_ptr(), None if offsets is None else offsets.data_ptr(),
          out.data_ptr(), ldo)
