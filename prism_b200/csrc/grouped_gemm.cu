@@ -6,26 +6,36 @@
 //   wgrad  dW[e][n, k] = sum over the expert's rows of dy[r, n] * x[r, k]
 //
 // One kernel in three modes on tcgen05.mma with fp32 accumulators in tensor memory, two CTAs to a tile (cta_group::2):
-//   * The weights' dimension (n, k, n) indexes the tile's 256 tensor-memory lanes, 128 in each CTA.  In fwd and dgrad the
-//     rows index its columns, so a tile of few rows is an MMA of few columns (a multiple of 32, chosen per tile): a group
-//     costs what its rows cost, rounded up to 32, and a group of one row still streams its matrix at full width.
+//   * The weights' dimension (n, k, n) indexes tensor-memory lanes, in blocks of 256 (128 in each CTA), one or two to a
+//     tile.  In fwd and dgrad the rows index the columns, so a tile of few rows is an MMA of few columns (a multiple of 32,
+//     chosen per tile): a group costs what its rows cost, and a group of one row still streams its matrix at full width.
 //   * Operands lie in shared memory as TMA writes them, in 128-byte swizzle spans: K-major where the contraction is
 //     contiguous in memory (x, W in fwd; dy in dgrad), MN-major where the other dimension is (W in dgrad, both in
 //     wgrad); the MMA takes either, so nothing is transposed.
-//   * Each CTA stages its own 128 lanes and half of the columns, 32 KB per 64 of the contraction.  With one CTA per tile
-//     (128 x 256, 48 KB for half the work) the kernel ran at the L2's limit: 16.4 TB/s into the SMs and 1351 TFLOP/s at
-//     32768 x 4096 x 4096 with 32 equal groups.
+//   * A tile of two lane blocks (512 x 256, four 48 KB stages) reads a quarter less per MMA than a tile of one (six 32 KB
+//     stages) and gives each load more MMA time to hide in: at the sizes below fwd 795 us against 989, dgrad 754 against
+//     1024, wgrad 879 against 1139.  One block serves where there are too few tiles, for groups of few rows (which stream
+//     their matrices and have no use for more MMA: 64 rows over 32 experts of 2048 x 4096 94 us against 109), and for fp32
+//     results, whose promotion below takes the registers.
+//   * The MMAs are issued by one elected lane of a warp that stays together, from descriptors kept as words: the issue
+//     must not take longer than the MMAs.
+//   * The epilogue moves an accumulator into registers, hands it back by an arrival that orders nothing else, and then
+//     stores.  (An arrival with .release also waits for the stores of the tile before: wgrad 879 -> 940 us.)
 //   * fwd and dgrad read past a group's last row into the next group's: those columns are computed and not stored.
 //     wgrad contracts over rows, so there the rows behind the group's last are overwritten with zeros in shared memory
 //     before the tile's last MMAs (both operands: a NaN there must not meet a zero).  Each CTA does so for its own
 //     stage, in warp 1; the second CTA's loads of such a stage complete on a barrier of its own, and its warp tells the
 //     first CTA, whose warp 1 issues all MMAs, when the zeros are in place.
-//   * wgrad to fp32: the tensor core adds with truncation, so a long sum drifts (2^-23 of a partial sum per step; 1.2e-6
-//     of the result's norm at 1000 rows).  Every 256 rows the accumulator is added to fp32 registers by the epilogue warps
-//     instead, while the MMAs go on into the other accumulator.
-//   * Warp 0 loads, warp 1 issues the MMAs, warps 2-9 store; two accumulators alternate.  Every wait is bounded as in
-//     gemm_bf16.cu.  Tiles are dealt round-robin to persistent CTA pairs; every CTA works out the groups' tiles from the
-//     offsets by itself (no launch before this one, no host copy of the offsets).
+//   * wgrad to fp32: the tensor core adds with truncation, so a long sum drifts (by up to 2^-23 of a partial sum per step;
+//     4.4e-6 of the result's norm at 4096 rows).  Every 512 rows the accumulator is added to fp32 registers by the epilogue
+//     warps instead (4.8e-7), while the MMAs go on into the other accumulator.
+//   * Warp 0 loads, warp 1 issues the MMAs, warps 2-17 store.  Every wait is bounded as in gemm_bf16.cu.  Tiles are dealt
+//     round-robin to persistent CTA pairs; every CTA works out the groups' tiles from the offsets by itself (no launch
+//     before this one, no host copy of the offsets).
+// Measured (CUDA events, cold L2, median of 40; the card is at its power limit, quartiles within 8%): 32768 rows,
+// 32 equal groups, 4096 x 4096: fwd 795 us (1384 TFLOP/s), dgrad 754, wgrad to bf16 879, to fp32 1200; uneven groups
+// (183 to 2237 rows) 884, 883, 951, 1262.  The dense kernel of gemm_bf16.cu takes 724 warm
+// on the first of these sizes, this one 742.
 // Offsets are read with care: each border is clamped to the rows that exist and to the border before it, so a wrong
 // array gives wrong products but no access outside the matrices.
 #include "common.cuh"
@@ -47,6 +57,7 @@ constexpr int EPI_WARPS = 16;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TMEM_COLS = 512;
 constexpr int MAX_EXPERTS = 1024;
+constexpr int GROUP_Q = 16;        // column tiles walked for each lane tile (L2 reuse); 4, 8 and 32 measure the same
 constexpr int PROMOTE_BLOCKS = 8;  // contraction blocks per accumulator of an fp32 wgrad
 constexpr uint32_t CHUNK_BYTES = 64 * 64 * 2;   // one 64 x 64 box
 constexpr uint32_t P_BYTES = HALF_P * BLOCK_C * 2;
@@ -68,7 +79,6 @@ struct Cfg {
     static constexpr uint32_t STAGE_BYTES = NB * P_BYTES + Q_BYTES;
     static constexpr int SIDES = NB == 1 ? 4 : 2;    // epilogue warps that share a lane quarter of a block
     static constexpr int HELD = 8 / SIDES;           // column blocks of 32 per epilogue warp
-    static constexpr int GROUP_Q = NB == 1 ? 8 : 16; // row tiles walked for each lane tile (L2 reuse), as in gemm_bf16.cu
     static_assert(STAGES * STAGE_BYTES == RING_BYTES, "both cuts fill the ring");
 };
 
@@ -90,7 +100,7 @@ __device__ __forceinline__ uint32_t desc_low(bool mn_major, uint32_t smem_addr) 
 }
 
 // One MMA of both CTAs.  Descriptors arrive as words so that a step along the contraction is one 32-bit addition: the
-// issuing thread has 128 cycles per MMA, and with 64-bit descriptors it needed more (700 cycles per 4 MMAs).
+// issuing thread has 128 cycles per MMA of 256 x 256 x 16.
 __device__ __forceinline__ void umma_pair(uint32_t tmem_d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t"
@@ -207,10 +217,9 @@ struct TileWalk {
             rows = group_rows(a, e);
             qt = (rows.y - rows.x + BLOCK_Q - 1) / BLOCK_Q;
         }
-        constexpr int GROUP = Cfg<NB>::GROUP_Q;
-        const int per_band = GROUP * p_tiles;
-        const int band = in / per_band, q_first = band * GROUP;
-        const int in_band = in - band * per_band, height = min(GROUP, qt - q_first);
+        const int per_band = GROUP_Q * p_tiles;
+        const int band = in / per_band, q_first = band * GROUP_Q;
+        const int in_band = in - band * per_band, height = min(GROUP_Q, qt - q_first);
         const int q = q_first + in_band % height;
         r.p0 = (in_band / height) * (NB * BLOCK_P);
         r.nb = NB == 1 || r.p0 + BLOCK_P < a.p_dim ? NB : 1;
@@ -221,8 +230,11 @@ struct TileWalk {
             r.blocks = (rows.y - rows.x + BLOCK_C - 1) / BLOCK_C;
             r.tail = (rows.y - rows.x) % BLOCK_C;
         } else {
-            r.q0 = rows.x + q * BLOCK_Q;
-            r.cols = min(BLOCK_Q, rows.y - r.q0);
+            // A group's rows in equal shares (multiples of 32 but for the last), not 256 at a time and a rest: the tiles'
+            // costs differ less (30000 x 2048 x 2048 over 60 uneven experts 227 -> 224 us, 32768 x 4096 x 4096 over 32 893 -> 884).
+            const int share = ((rows.y - rows.x + qt - 1) / qt + 31) & ~31;
+            r.q0 = rows.x + q * share;
+            r.cols = min(share, rows.y - r.q0);
             r.first = 0;
             r.blocks = (a.c_dim + BLOCK_C - 1) / BLOCK_C;
             r.tail = 0;
@@ -585,8 +597,7 @@ grouped_gemm_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap map
             if (timed_out) break;
             if (MODE == WGRAD) {
                 // A lane holds consecutive columns of one row of dW.  16 rows x 128 bytes at a time pass through the warp's
-                // 2 KB of shared memory (16-byte pieces XOR-swizzled by row), so that stores write whole lines: 64-byte
-                // pieces reached 4.9 TB/s on empty groups where a fill reaches 7.2.
+                // 2 KB of shared memory (16-byte pieces XOR-swizzled by row), so that stores write whole lines.
                 constexpr int PIECE = 16 / sizeof(Out);
                 unsigned char* buf = epi_smem + (warp - 2) * 2048;
 #pragma unroll
@@ -726,10 +737,10 @@ int launch_grouped(const GroupedArgs& a, long long most_tiles, const CUtensorMap
 
 long long tiles_of(int p_dim, int blocks) { return (p_dim + blocks * gg::BLOCK_P - 1) / (blocks * gg::BLOCK_P); }
 
-// One or two lane blocks per tile, by the rounds of tiles that the 74 CTA pairs make.  A tile of two blocks costs 1.55 of
-// a tile of one (1030 and 670 cycles per 64 of the contraction), but small problems have too few of them: measured at
-// 5003 x 1000 x 2056 over 9 experts 61 us with two blocks and 55 with one, at 32768 x 4096 x 4096 over 32 uneven experts
-// 795 and 899.
+// One or two lane blocks per tile, by the rounds of tiles that the 74 CTA pairs make, with a tile of two at 1.55 of a tile
+// of one (2 x 754/1024 to 2 x 795/989 at the sizes above).  Over 36 drawn problems (1500 to 30000 rows, 4 to 60 experts,
+// matrices of 400 to 5600) the choice is 1.3% behind the better of the two on average and 25% at worst (2637 rows, 9
+// experts, 1224 x 1560: 30.7 us with two, 24.6 with one); always one would be 8% behind, always two 4%.
 bool two_blocks(int p_dim, long long q_tiles) {
     constexpr long long PAIRS = 74;
     const long long t1 = tiles_of(p_dim, 1) * q_tiles, t2 = tiles_of(p_dim, 2) * q_tiles;
