@@ -23,11 +23,11 @@ def weights(lead, n, k, group, dtype, zeros, seed, exact=False):
 
 
 def dense(q, scales, z, group):
-    """scales * (q - z) in fp64, the group's scale and zero point repeated; and scales * (32 + q + z)."""
+    """scales * (q - z) in fp64, the group's scale and zero point repeated."""
     v = torch.stack([q & 15, q >> 4], dim=-1).flatten(-2).double()
     s = scales.double().repeat_interleave(group, -1)
     zz = torch.full_like(s, 8.0) if z is None else z.double().repeat_interleave(group, -1)
-    return s * (v - zz), s * (v + zz + 32)
+    return s * (v - zz)
 
 
 def check(pb, sizes, spare, n, k, group, dtype, zeros, seed=0, exact=False, grouped=True):
@@ -38,20 +38,20 @@ def check(pb, sizes, spare, n, k, group, dtype, zeros, seed=0, exact=False, grou
     x = (torch.randint(-2, 3, (rows, k), device=DEV, generator=g) if exact else torch.randn((rows, k), device=DEV, generator=g)).to(dtype)
     out = torch.full((rows, n), 7.0, dtype=dtype, device=DEV)
     got = pb.gemv_w4(x, q, scales, zeros=z, offsets=borders(sizes) if grouped else None, out=out)
-    w, big = dense(q, scales, z, group)
+    w = dense(q, scales, z, group)
     want = torch.full((rows, n), 7.0, dtype=torch.float64, device=DEV)
-    size, terms = torch.zeros_like(want), torch.zeros_like(want)
+    terms = torch.zeros_like(want)
     at = 0
     for e, s in enumerate(sizes):
         r = slice(at, at + s)
-        we, be = (w[e], big[e]) if grouped else (w, big)
-        want[r], terms[r], size[r] = x[r].double() @ we.t(), x[r].double().abs() @ we.abs().t(), x[r].double().abs() @ be.t()
+        we = w[e] if grouped else w
+        want[r], terms[r] = x[r].double() @ we.t(), x[r].double().abs() @ we.abs().t()
         at += s
     if exact:   # integers times powers of two: all fp32 sums are exact
         assert torch.equal(got, want.to(dtype)), (sizes, n, k, group)
         return
-    # a group's sums of (16 + q) x and (16 + z) x: one step of a partial sum per addition; then the groups' additions
-    fp32 = (group + 2) * 2.0 ** -23 * size + (k // group + 8) * 2.0 ** -24 * terms
+    # the products are exact; one step of a partial sum per addition inside a group, half a step for the groups' additions
+    fp32 = ((group + 2) * 2.0 ** -23 + (k // group + 20) * 2.0 ** -24) * terms
     half_step, least = (2.0 ** -8, 0.0) if dtype == BF else (2.0 ** -11, 2.0 ** -25)
     assert ((got.double() - want).abs() <= fp32 + half_step * (want.abs() + fp32) + least).all(), (sizes, n, k, group)
 
