@@ -20,7 +20,7 @@ constexpr int MAX_EXPERTS = 1024;
 constexpr int MAX_CHOICES = 32;    // lane j of a token's warp holds its choice j
 constexpr int CHUNK = 128;         // tokens whose choices a block ranks at a time
 constexpr int WORDS = CHUNK / 32;
-constexpr int ONE_BLOCK = 64;      // tokens up to which one block makes the whole order: 128 took 7.4 us, 5.2 in two launches
+constexpr int ONE_BLOCK = 64;      // tokens up to which one block makes the whole order: 128 (of 128 experts, 8 choices) take 12.8 us, 7.3 in two launches
 constexpr int MAX_BLOCKS = 148;    // one block of 32 warps per SM
 constexpr unsigned FULL = 0xffffffffu;
 }  // namespace rt

@@ -89,10 +89,16 @@ def test_masks(pb):
     r = check_route(pb, l, 2, True)
     assert (r.ids[:, 0] == 7).all() and (r.ids[:, 1] == 0).all()
     check_route(pb, torch.full((3, 20), lowest, device=DEV), 4, False)
-    l = make_logits(150, 24, torch.float32, 10)          # NaN is passed over
-    l[torch.rand_like(l) < 0.3] = float("nan")
-    check_route(pb, l, 5, True)
-    check_route(pb, l, 5, False)
+    for dtype in DTYPES.values():                        # NaN is passed over
+        for experts in (24, 100, 300):
+            l = make_logits(150, experts, torch.float32, 10, 0.1)
+            l[torch.rand_like(l) < 0.3] = float("nan")
+            check_route(pb, l.to(dtype), 5, True)
+            check_route(pb, l.to(dtype), 5, False)
+        low = torch.full((90, 40), torch.finfo(dtype).min, dtype=dtype, device=DEV)
+        low[:, 30] = torch.finfo(dtype).max
+        r = check_route(pb, low, 2, True) if dtype != torch.float32 else pb.route_topk(low, 2)   # max - min overflows fp32: weights 1, 0
+        assert (r.ids[:, 0] == 30).all() and (r.ids[:, 1] == 0).all() and (r.weights[:, 0] == 1).all()
 
 
 def test_strided_logits_given_outputs_and_workspace(pb):
