@@ -131,16 +131,16 @@ def route_topk(logits: torch.Tensor, k: int, renormalize: bool = True, out=None,
         _tensor("order", out.order, device, torch.int32, (tokens * k,))
         _tensor("offsets", out.offsets, device, torch.int32, (experts + 1,))
     need = route_workspace_size(tokens, experts, k)
-    if workspace is None:
-        scratch = torch.empty(need, dtype=torch.uint8, device=device).data_ptr() if need else None
+    if workspace is None:   # kept until both launches are queued: whoever gets its memory next comes behind them
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     else:
         if not isinstance(workspace, torch.Tensor) or workspace.device != device or not workspace.is_contiguous():
             raise ValueError("workspace must be a contiguous tensor on the device of logits")
         if workspace.numel() * workspace.element_size() < need:
             raise ValueError("workspace too small; see route_workspace_size(tokens, experts, k)")
-        scratch = workspace.data_ptr() if need else None
     _run(device, load().prism_b200_route_topk, tokens, experts, k, code, logits.data_ptr(), ld, int(bool(renormalize)),
-         out.ids.data_ptr(), out.weights.data_ptr(), out.pos.data_ptr(), out.order.data_ptr(), out.offsets.data_ptr(), scratch)
+         out.ids.data_ptr(), out.weights.data_ptr(), out.pos.data_ptr(), out.order.data_ptr(), out.offsets.data_ptr(),
+         workspace.data_ptr() if need else None)
     return out
 
 

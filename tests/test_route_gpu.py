@@ -319,3 +319,21 @@ def test_refusals(pb):
         pb.route_topk_grad(logits, r.ids, r.weights[:3], r.weights)
     with pytest.raises(pb.PrismB200Error):
         pb.route_topk_grad(logits, r.ids, r.weights, r.weights, out=logits)
+
+
+def test_own_scratch_lives_until_the_call_is_queued(pb, monkeypatch):
+    """Memory that another thread allocates while the launches are queued is not the call's own scratch."""
+    from prism_b200 import experts
+    inner, seen = experts._run, []
+
+    def run(device, fn, *args):
+        other = torch.empty(pb.route_workspace_size(500, 64, 4), dtype=torch.uint8, device=device)
+        seen.append((args[-1], other.data_ptr()))
+        inner(device, fn, *args)
+
+    logits = make_logits(500, 64, torch.float32, 3)
+    pb.route_topk(logits, 4)   # leaves a block of that size with the allocator
+    monkeypatch.setattr(experts, "_run", run)
+    pb.route_topk(logits, 4)
+    (scratch, other), = seen
+    assert scratch and scratch != other
