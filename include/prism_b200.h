@@ -308,7 +308,9 @@ int prism_b200_gemm_bf16_fill_mode(int mode);
  *
  * Row matrices are given by a pointer, a width and a row stride `ld` in elements (ld >= width); rows are contiguous
  * inside.  Outputs must not overlap inputs.  Every call is one launch (route_topk: two above 64 tokens), results
- * repeat bit for bit, and calls on several streams at once need only outputs (and workspaces) of their own.
+ * repeat bit for bit, and calls on several streams at once need only outputs (and workspaces) of their own: two captured
+ * graphs that may run at the same time must not share them.  Everything can be captured; the first grouped or 4-bit
+ * product on a device registers the library's error word there, so make one such call before a capture.
  */
 
 /* Element types of the entry points that take one. */
@@ -341,7 +343,8 @@ int prism_b200_route_topk_grad(int tokens, int experts, int k, int dtype, const 
 
 /*
  * out[pos[t][j]] = x[t] (`rows` rows of out exist; a position outside them is passed over, other rows stay as they
- * are).  Its gradient is prism_b200_route_combine without weights.
+ * are).  The positions are distinct, as route_topk's are; of several that name one row any may win.  Its gradient is
+ * prism_b200_route_combine without weights.
  */
 int prism_b200_route_gather(int dtype, int tokens, int k, int width, const void* x, long long ldx, const int* pos, long long rows,
                             void* out, long long ldo, void* stream);
@@ -352,7 +355,7 @@ int prism_b200_route_combine(int dtype, int tokens, int k, int width, const void
 
 /*
  * Gradient of prism_b200_route_combine: dy[pos[t][j]] = weights[t][j] * dout[t] (other rows of dy stay as they are),
- * dweights[t][j] = dot(dout[t], y[pos[t][j]]) (0 where there is no row).  The positions are distinct.
+ * dweights[t][j] = dot(dout[t], y[pos[t][j]]) (0 where there is no row).  The positions are distinct here too.
  */
 int prism_b200_route_combine_grad(int dtype, int tokens, int k, int width, const void* dout, long long ldd, const void* y,
                                   long long ldy, long long rows, const int* pos, const float* weights, void* dy, long long lddy,

@@ -20,7 +20,7 @@
 //     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
 //     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
 //   * The team's sums meet in shared memory once per item, added in warp order.
-// What bounds it now: at 16384 x 16384 and one row 39 us, where the copies alone take 25 and the arithmetic alone 31 (shifts
+// Where the time goes: at 16384 x 16384 and one row 39 us, where the copies alone take 25 and the arithmetic alone 31 (shifts
 // and masks on the half-rate ALU pipe and mma.sync at 16 cycles per instruction and scheduler take about 22 each).
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -49,7 +49,8 @@ constexpr int SMEM_BYTES = 232448;
 // Shared memory: rings (512-byte aligned), scales (two blocks per warp), sums of the warps (two sets), barriers, flags, tables.
 struct Layout {
     int xrows, stage, stages, red_floats, scales, red, bars, bytes;
-    __host__ __device__ Layout(int rows, int experts) {
+    __host__ __device__ constexpr Layout(int rows, int experts)
+        : xrows(0), stage(0), stages(0), red_floats(0), scales(0), red(0), bars(0), bytes(0) {
         xrows = rows < COLS ? rows : COLS;
         stage = W_BYTES + (xrows * X_PITCH + 511) / 512 * 512;
         red_floats = xrows * RED_PITCH;
@@ -62,6 +63,7 @@ struct Layout {
         bytes = rest + scales;
     }
 };
+static_assert(Layout(COLS, MAX_EXPERTS).stages >= 2, "a copy is in flight while a slice is used, at the largest sizes too");
 }  // namespace w4
 
 // (a & b) | c in one instruction.

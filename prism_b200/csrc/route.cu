@@ -60,8 +60,9 @@ template <typename T> __device__ __forceinline__ float packed_value(uint32_t key
     return to_f32(*reinterpret_cast<const T*>(&b));
 }
 
-// The k choices of one token by one warp (row: its logits of experts lane, lane + 32, ...): lane j < k returns its choice's expert (-1: none) and logit, every lane the
-// largest logit and, with `all`, this lane's share of the sum of exp(logit - largest) over all experts.
+// The k choices of one token by one warp (row: its logits of experts lane, lane + 32, ...): lane j < k returns its
+// choice's expert (-1: none) and logit, every lane the largest logit and, with `all`, this lane's share of the sum of
+// exp(logit - largest) over all experts.
 // A round takes the largest key of the lanes' best (redux.sync); the lane that has it goes on to its next.  Lanes with up
 // to eight keys sort them first, so that this is a shift; others look through their keys again.
 template <typename T, int EPL>
@@ -223,9 +224,10 @@ __device__ __forceinline__ int warp_exclusive_scan(const int* count, int* base, 
     return carry;
 }
 
-// One warp per token (choose).  Then the block ranks its choices: a token chooses an expert at most once, so a bit per (expert, token) says everything, and the rank
-// of a choice is a popcount of the bits of earlier tokens.  With one block (grid 1, tokens <= ONE_BLOCK) the order is
-// complete here; otherwise the ranks are relative to the block and route_place_kernel adds the rest.
+// One warp per token (choose).  Then the block ranks its choices: a token chooses an expert at most once, so a bit per
+// (expert, token) says everything, and the rank of a choice is a popcount of the bits of earlier tokens.  With one block
+// (grid 1, tokens <= ONE_BLOCK) the order is complete here; otherwise the ranks are relative to the block and
+// route_place_kernel adds the rest.
 template <typename T, int EPL>
 __global__ void __launch_bounds__(1024, 1) route_choose_kernel(RouteArgs a) {
     using namespace rt;

@@ -7,12 +7,13 @@ with 4-bit weights.
     y = route_combine(ys, r.pos, r.weights)                  # back into token order, weighted and added up
 
 and their gradients: route_combine_grad, grouped_gemm_bf16_dgrad and _wgrad, route_combine without weights (of the
-gather) and route_topk_grad.  How many rows an expert gets stays on the device, so all of this can run without a host
-synchronisation and be captured in a CUDA graph.  Everything runs on the current stream of the tensors' device through
-the C ABI in include/prism_b200.h, which states the operators in full; nothing falls back to PyTorch.
+gather) and route_topk_grad.  They are called by name: nothing is recorded for autograd.  How many rows an expert gets
+stays on the device, so all of this can run without a host synchronisation and be captured in a CUDA graph (after one
+grouped or 4-bit product on the device).  Everything runs on the current stream of the tensors' device through the C ABI
+in include/prism_b200.h, which states the operators in full; nothing falls back to PyTorch.
 
 A row matrix is a 2-D tensor whose rows are contiguous (its row stride may be larger than its width).  Buffers made for
-tokens * k rows hold their groups in front; what lies behind offsets[-1] is neither read nor written.
+tokens * k rows hold their groups in front; what lies behind offsets[-1] does not matter and is not written.
 """
 from __future__ import annotations
 

@@ -77,6 +77,8 @@ def test_w4_refusals(lib):
     assert call(dtype=0) == 1 and call(rows=-1) == 1 and call(experts=2) == 1 and call(x=None) == 1 and call(ldx=128) == 1
     assert call(group=16) == 2 and call(k=200) == 2 and call(k=0) == 2 and call(experts=1025, offsets=P) == 2
     assert call(x=ODD) == 3 and call(ldx=260) == 3 and call(q=ODD) == 3
+    assert call() == 1 and "overlap" in _lib.last_error()[1]
+    assert call(ldo=63) == 1 and call(scales=ctypes.c_void_p((1 << 20) + 1)) == 3
 
 
 def test_python_layer_has_no_cpu_path():
