@@ -307,7 +307,7 @@ int prism_b200_gemm_bf16_fill_mode(int mode);
  * the device: the products read the group borders (`offsets`) there, and nothing is copied to the host.
  *
  * Row matrices are given by a pointer, a width and a row stride `ld` in elements (ld >= width); rows are contiguous
- * inside.  Outputs must not overlap inputs.  Every call is one launch (route_topk: two above 64 tokens), results
+ * inside; widths, n and k are at most 2^30.  Outputs must not overlap inputs.  Every call is one launch (route_topk: two above 64 tokens), results
  * repeat bit for bit, and calls on several streams at once need only outputs (and workspaces) of their own: two captured
  * graphs that may run at the same time must not share them.  Everything can be captured; the first grouped or 4-bit
  * product on a device registers the library's error word there, so make one such call before a capture.

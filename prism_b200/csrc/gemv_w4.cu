@@ -537,8 +537,8 @@ extern "C" int prism_b200_gemv_w4(int dtype, int rows, int experts, int n, int k
     if (rows == 0 || n == 0 || experts == 0) return PRISM_B200_OK;
     if (k == 0) return set_error(PRISM_B200_ERR_UNSUPPORTED_SHAPE, "gemv_w4: nothing to add up (k is 0)");
     if (!x || !q || !scales || !out) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "gemv_w4: null pointer");
-    if ((n + 31LL) / 32 * (rows + static_cast<long long>(experts)) > 0x3fffffffLL)
-        return set_error(PRISM_B200_ERR_TOO_LARGE, "gemv_w4: too many tiles");
+    if (rows > 1 << 30 || n > 1 << 30 || k > 1 << 30 || (n + 31LL) / 32 * (rows + static_cast<long long>(experts)) > 0x3fffffffLL)
+        return set_error(PRISM_B200_ERR_TOO_LARGE, "gemv_w4: a size above 2^30 or too many tiles");
     if (ldx < k || ldo < n) return set_error(PRISM_B200_ERR_INVALID_ARGUMENT, "gemv_w4: a row stride below the row's width");
     if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(q)) & 15u || ldx % 8)
         return set_error(PRISM_B200_ERR_MISALIGNED, "gemv_w4: x and q must be 16-byte aligned, x's row stride a multiple of 8");

@@ -757,7 +757,7 @@ int check_grouped(const char* fn, int experts, int rows, int n, int k, bool* don
         return set_error(PRISM_B200_ERR_UNSUPPORTED_SHAPE, "%s: need n %% 8 == 0 and k %% 8 == 0 (got %d, %d)", fn, n, k);
     if (experts == 0) *done = true;
     const long long tiles = ((n > k ? n : k) / 64LL + 1) * (rows / 64LL + experts) , wtiles = (n / 128LL + 1) * (k / 128LL + 1) * experts;
-    if (rows > 1 << 30 || tiles > 0x3fffffffLL || wtiles > 0x3fffffffLL) return set_error(PRISM_B200_ERR_TOO_LARGE, "%s: too many tiles", fn);
+    if (rows > 1 << 30 || n > 1 << 30 || k > 1 << 30 || tiles > 0x3fffffffLL || wtiles > 0x3fffffffLL) return set_error(PRISM_B200_ERR_TOO_LARGE, "%s: a size above 2^30 or too many tiles", fn);
     return PRISM_B200_OK;
 }
 

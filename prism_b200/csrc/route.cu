@@ -808,6 +808,7 @@ int check_copy(const char* fn, int dtype, int tokens, int k, int width, long lon
         return set_error(PRISM_B200_ERR_UNSUPPORTED_SHAPE, "%s: 1 to %d choices (got %d)", fn, rt::MAX_CHOICES, k);
     if (static_cast<long long>(tokens) * k > 1LL << 30)
         return set_error(PRISM_B200_ERR_TOO_LARGE, "%s: tokens x k at most 2^30", fn);
+    if (width > 1 << 30) return set_error(PRISM_B200_ERR_TOO_LARGE, "%s: rows of at most 2^30 elements", fn);
     if (int rc = check_rows(fn, ld_a, width)) return rc;
     return check_rows(fn, ld_b, width);
 }

@@ -125,3 +125,68 @@ def test_wrong_device_is_refused(pb):
         pb.route_gather(x.cpu(), r.pos)
     with pytest.raises(TypeError):
         pb.grouped_gemm_bf16(x, w1, r.offsets.cpu())
+
+
+def ints(shape, seed, dtype=BF):
+    return torch.randint(-3, 4, shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)).to(dtype)
+
+
+def test_matrices_past_32_bits(pb):
+    """150 matrices of 4096 x 4096 (2.5 G elements, 5 GB); the first, one past 2^31 elements and the last have rows."""
+    E, n = 150, 4096
+    used, sizes = (0, 129, E - 1), [0] * E
+    for e, s in zip(used, (3, 40, 5)):
+        sizes[e] = s
+    offsets = torch.tensor([0] + sizes, device=DEV).cumsum(0).to(torch.int32)
+    x, dy = ints((48, n), 1), ints((48, n), 2)
+    w = torch.empty((E, n, n), dtype=BF, device=DEV)
+    for e in used:
+        w[e] = ints((n, n), 10 + e)
+    groups = [(e, slice(int(offsets[e]), int(offsets[e + 1]))) for e in used]
+    out, dx = pb.grouped_gemm_bf16(x, w, offsets), pb.grouped_gemm_bf16_dgrad(dy, w, offsets)
+    for e, r in groups:   # integers below 2^24: fp32 sums are exact, one rounding
+        assert torch.equal(out[r], (x[r].double() @ w[e].double().t()).to(BF)) and torch.equal(dx[r], (dy[r].double() @ w[e].double()).to(BF))
+    for dtype in (BF, torch.float32):
+        dw = torch.full((E, n, n), 7.0, dtype=dtype, device=DEV)
+        pb.grouped_gemm_bf16_wgrad(dy, x, offsets, out=dw)
+        for e, r in groups:
+            assert torch.equal(dw[e], (dy[r].double().t() @ x[r].double()).to(dtype))
+        assert not dw[130:E - 1].any() and not dw[1:129].any()
+
+
+def test_4_bit_matrices_past_32_bits(pb):
+    """1024 matrices of 4104 x 2048 (4.3 GB of weights, offsets past 2^32 bytes)."""
+    E, n, k, group = 1024, 4104, 2048, 128
+    sizes = [0] * E
+    sizes[1], sizes[700], sizes[E - 1] = 2, 9, 1
+    offsets = torch.tensor([0] + sizes, device=DEV).cumsum(0).to(torch.int32)
+    q = torch.empty((E, n, k // 2), dtype=torch.uint8, device=DEV)
+    scales = torch.ones((E, n, k // group), dtype=BF, device=DEV)
+    x = ints((12, k), 3)
+    for e in (1, 700, E - 1):
+        q[e] = torch.randint(0, 256, (n, k // 2), device=DEV, generator=torch.Generator(device=DEV).manual_seed(e)).to(torch.uint8)
+        scales[e, :, ::2] = 0.5
+    got = pb.gemv_w4(x, q, scales, offsets=offsets)
+    for e in (1, 700, E - 1):
+        r = slice(int(offsets[e]), int(offsets[e + 1]))
+        v = torch.stack([q[e] & 15, q[e] >> 4], -1).flatten(-2).double() - 8
+        assert torch.equal(got[r], (x[r].double() @ (v * scales[e].double().repeat_interleave(group, -1)).t()).to(BF))
+
+
+def test_rows_past_32_bits(pb):
+    """Buffers of 2.4 G elements: rows at both ends."""
+    T, k, H, rows = 37, 3, 4096, 590_000
+    x, weights = ints((T, H), 4), (ints((T, k), 5, torch.float32) / 4)
+    pos = torch.randperm(T * k, device=DEV, generator=torch.Generator(device=DEV).manual_seed(6)).to(torch.int32).view(T, k)
+    pos = torch.where(pos < 50, pos, rows - T * k + pos).contiguous()
+    at = pos.long()
+    y = torch.full((rows, H), 7.0, dtype=BF, device=DEV)
+    pb.route_gather(x, pos, out=y)
+    assert torch.equal(y[at], x[:, None].expand(T, k, H)) and bool((y[50:rows - T * k + 50] == 7.0).all())
+    y[at] = ints((T, k, H), 7)
+    assert torch.equal(pb.route_combine(y, pos, weights), (weights[:, :, None].double() * y[at].double()).sum(1).to(BF))
+    dy = torch.full((rows, H), 7.0, dtype=BF, device=DEV)
+    _, dweights = pb.route_combine_grad(x, y, pos, weights, dy=dy)
+    assert torch.equal(dy[at], (weights[:, :, None] * x[:, None].float()).to(BF))
+    assert torch.equal(dweights, (y[at].double() * x[:, None].double()).sum(2).float())
+    assert bool((dy[50:rows - T * k + 50] == 7.0).all())

@@ -47,6 +47,10 @@ def test_route_refusals(lib):
     assert lib.prism_b200_route_combine(1, 0, 2, 64, None, 64, 0, None, None, None, 64, None) == 0
     assert lib.prism_b200_route_combine(1, 4, 33, 64, P, 64, 8, P, None, P, 64, None) == 2
     assert lib.prism_b200_route_combine_grad(1, 4, 2, 64, P, 64, P, 64, 8, P, P, P, 64, P, None) == 1
+    big = (1 << 30) + 8
+    assert lib.prism_b200_route_gather(1, 4, 2, big, P, big, P, 8, P, big, None) == 6
+    assert lib.prism_b200_route_combine(1, 4, 2, big, P, big, 8, P, None, P, big, None) == 6
+    assert lib.prism_b200_route_combine_grad(1, 4, 2, big, P, big, P, big, 8, P, P, P, big, P, None) == 6
     assert lib.prism_b200_route_combine_grad(1, 1 << 29, 4, 64, P, 64, P, 64, 8, P, P, P, 64, P, None) == 6
 
 
@@ -64,6 +68,9 @@ def test_grouped_refusals(lib):
     assert f(2, 8, 64, 64, P, 56, P, P, P, 64, None) == 1
     assert f(2, 8, 64, 64, P, 64, P, P, P, 64, None) == 1 and "overlap" in _lib.last_error()[1]
     assert f(1024, 1 << 30, 1 << 20, 64, P, 64, P, P, P, 1 << 20, None) == 6
+    big = (1 << 30) + 8
+    assert f(1, 1, 8, big, P, big, P, P, P, 8, None) == 6 and d(1, 1, big, 8, P, big, P, P, P, 8, None) == 6
+    assert w(1, 1, 8, big, P, 8, P, big, P, 1, P, None) == 6
     assert d(2, 8, 0, 64, P, 0, P, P, P, 64, None) == 2
     assert w(2, 8, 64, 64, P, 64, P, 64, P, 2, P, None) == 1                                      # fp16 result
     assert w(2, 8, 64, 64, P, 64, P, 64, P, 0, P, None) == 1 and "overlap" in _lib.last_error()[1]
@@ -78,6 +85,8 @@ def test_w4_refusals(lib):
     assert call(group=16) == 2 and call(k=200) == 2 and call(k=0) == 2 and call(experts=1025, offsets=P) == 2
     assert call(x=ODD) == 3 and call(ldx=260) == 3 and call(q=ODD) == 3
     assert call() == 1 and "overlap" in _lib.last_error()[1]
+    big = (1 << 30) + 128
+    assert call(k=big, ldx=big) == 6 and call(n=big, ldo=big) == 6 and call(rows=big) == 6
     assert call(ldo=63) == 1 and call(scales=ctypes.c_void_p((1 << 20) + 1)) == 3
 
 
