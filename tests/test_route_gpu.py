@@ -337,3 +337,49 @@ def test_own_scratch_lives_until_the_call_is_queued(pb, monkeypatch):
     pb.route_topk(logits, 4)
     (scratch, other), = seen
     assert scratch and scratch != other
+
+
+@pytest.mark.parametrize("E,k", [(8, 8), (64, 8), (256, 3)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_every_16_bit_pattern(pb, dtype, E, k):
+    """All 65536 patterns, several times among others: both zeros, subnormals, infinities and NaNs."""
+    g = torch.Generator(device=DEV).manual_seed(E)
+    bits = torch.cat([torch.randperm(1 << 16, device=DEV, generator=g) for _ in range(4)])
+    logits = bits.to(torch.int32).sub(1 << 15).to(torch.int16).view(DTYPES[dtype]).view(-1, E)
+    ids, _, pos, order, offsets = plain_route(logits, k, True)
+    r = pb.route_topk(logits, k)
+    for name, want in (("ids", ids), ("pos", pos), ("order", order), ("offsets", offsets)):
+        assert np.array_equal(getattr(r, name).cpu().numpy(), want), name
+
+
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("T,E,k", [(3, 8, 1), (64, 40, 8), (70, 64, 4), (999, 128, 8), (4801, 504, 7), (300, 1024, 8)])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_16_bit_logits_in_vectors_or_not(pb, dtype, T, E, k, renorm):
+    """Whole 16-byte vectors take another way than rows at odd strides; both make the same choice."""
+    logits = make_logits(T, E, DTYPES[dtype], T, 0.2)
+    logits[::7] = logits[::7].round()   # ties
+    check_route(pb, logits, k, renorm)
+    odd = torch.zeros((T, E + 3), dtype=DTYPES[dtype], device=DEV)[:, 1:E + 1]
+    odd.copy_(logits)
+    a, b = pb.route_topk(logits, k, renormalize=renorm), pb.route_topk(odd, k, renormalize=renorm)
+    for name in ("ids", "pos", "order", "offsets"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+
+
+def test_blocks_of_more_tokens_than_16_bits_count(pb):
+    """65537 tokens per block: the counts between the launches are 32 bits wide."""
+    T, E = 148 * 65536 + 5, 3
+    logits = torch.randn((T, E), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    logits[:, 2] -= 30.0   # so that a block has more than 65535 rows of one expert
+    logits[: 3 * 65536, 0] += 60.0
+    r = pb.route_topk(logits, 1)
+    ids = logits.argmax(1)
+    assert torch.equal(r.ids[:, 0].long(), ids) and bool((r.weights == 1).all())
+    counts = torch.bincount(ids, minlength=E)
+    assert torch.equal(r.offsets.long(), torch.cat([counts.new_zeros(1), counts.cumsum(0)]))
+    rows = torch.sort(ids, stable=True).indices
+    assert torch.equal(r.order.long(), rows)
+    want = torch.empty_like(rows)
+    want[rows] = torch.arange(T, device=DEV)
+    assert torch.equal(r.pos[:, 0].long(), want)
