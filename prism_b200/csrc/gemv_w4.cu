@@ -7,9 +7,11 @@
 // 23 bytes (46 weights) per clock to keep up with HBM.
 //   * Products and sums are mma.sync m16n8k16 with fp32 accumulators: 16 weight rows x 16 k against up to 8 rows of x.
 //     tcgen05 would want the converted weights in shared memory, a round trip of four times the bytes read here.
-//   * A nibble becomes an operand by one shift and one LOP3, which put it into the mantissa of 16.0 (bf16) or 64.0 (fp16),
-//     and one packed subtraction of 16 + z: q - z, exactly.  So the products are exact and only the sums round, in fp32.
-//     (Taking the base and z off afterwards, with sum x from one more MMA, took the same time and costs bits.)
+//   * Nibbles become operands where they lie in a byte, two bytes at a time: by one AND or LOP3 and one packed FMA or
+//     subtraction that leaves q - z (bf16: times 2^-7), exactly; a word needs one shift.  So the products are exact and
+//     only the sums round, in fp32.  (One base for all nibbles takes three shifts and a multiplication, bf16, or one and
+//     two, fp16: 39 us at 16384 x 16384 where this takes 36 for both types; shifts as high halves of products 42 to 44; base and z
+//     taken off afterwards with sum x from one more MMA no less, and it costs bits.)
 //   * A 32-bit word holds 8 consecutive k; the MMA's order of k is free as long as both operands follow it, so the
 //     pairs are (k, k + 4) as the masks deliver them, and x is brought into that order by four PRMTs per 8 values.
 //   * The four lanes of a quad take one, two or four consecutive words each, 32, 64 or 128 k together: a group, whose sum is
@@ -20,10 +22,9 @@
 //     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
 //     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
 //   * The team's sums meet in shared memory once per item, added in warp order.
-// Where the time goes: 16384 x 16384, one row, takes 39 us; the copies alone take 25 and the arithmetic alone 31.  On the
-// SMs at work the ALU pipe (shifts and masks, at half rate) is 74% busy and the schedulers issue in 75% of the cycles; the
-// tensor pipe, an mma.sync taking it 8 cycles per scheduler, is at 27%.  512 tiles in teams of four warps use 128 of the
-// 148 SMs: 18944 rows, which use all, take the same time (4.0 TB/s).
+// Where the time goes: 16384 x 16384, one row, takes 36 us; the copies alone take 25.  On the SMs at work the schedulers
+// issue in 70% of the cycles and the ALU pipe is 66% busy; the tensor pipe, an mma.sync taking it 8 cycles per scheduler,
+// is at 30%.  512 tiles in teams of four warps use 128 of the 148 SMs: 18944 rows, which use all, take 37 us (4.3 TB/s).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -77,17 +78,18 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
 
 template <typename T> struct W4Type;
 template <> struct W4Type<__nv_bfloat16> {
-    static constexpr uint32_t EIGHT = 0x41C041C0u;   // 16 + 8, twice
-    // 16 + z, twice
-    static __device__ __forceinline__ uint32_t zero(uint32_t z) { return (z << 3) * 0x10001u | 0x41804180u; }
-    static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-        const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-        return *reinterpret_cast<const uint32_t*>(&d);
+    static constexpr float UNIT = 128.f;   // operands are (q - z) / 128
+    // An integer in the lowest eight bits of a bf16 is itself times 2^-133, through the subnormals and the first normal
+    // numbers; so both nibbles of a byte serve where they lie, and one FMA scales them and takes z off, exactly.
+    template <int ODD> static __device__ __forceinline__ uint32_t zero(uint32_t z) { return ODD ? 0u : fma(z * 0x10001u, 0xFE80FE80u, 0u); }
+    template <int I> static __device__ __forceinline__ uint32_t operand(uint32_t w, uint32_t even, uint32_t odd) {
+        const uint32_t s = I < 2 ? w : w >> 8;
+        return I & 1 ? fma(s & 0x00F000F0u, 0x7C807C80u, even) : fma(s & 0x000F000Fu, 0x7E807E80u, even);   // 2^122, 2^126
     }
-    // nibble i of the word's two halves -> (16 + q) twice: 16.0 is 0x4180, the mantissa's top four bits are bits 3-6
-    template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-        const uint32_t s = I == 0 ? w * 8u : w >> (4 * I - 3);
-        return and_or(s, 0x00780078u, 0x41804180u);
+    static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
     }
     // d = a * b + d, or a * b where FIRST (no registers to clear before a group's first step)
     template <bool FIRST>
@@ -106,17 +108,19 @@ template <> struct W4Type<__nv_bfloat16> {
     static __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct W4Type<__half> {
-    static constexpr uint32_t EIGHT = 0x54805480u;   // 64 + 8, twice
-    static __device__ __forceinline__ uint32_t zero(uint32_t z) { return (z << 4) * 0x10001u | 0x54005400u; }   // 64 + z, twice
+    static constexpr float UNIT = 1.f;
+    // 1024.0 is 0x6400 and counts bits 0-3 of its mantissa in ones, 64.0 is 0x5400 and counts bits 4-7: both nibbles of a
+    // byte become 1024 + q or 64 + q where they lie, and 1024 + z or 64 + z is taken off.
+    template <int ODD> static __device__ __forceinline__ uint32_t zero(uint32_t z) {
+        return ODD ? (z << 4) * 0x10001u | 0x54005400u : z * 0x10001u | 0x64006400u;
+    }
+    template <int I> static __device__ __forceinline__ uint32_t operand(uint32_t w, uint32_t even, uint32_t odd) {
+        const uint32_t s = I < 2 ? w : w >> 8;
+        return I & 1 ? sub(and_or(s, 0x00F000F0u, 0x54005400u), odd) : sub(and_or(s, 0x000F000Fu, 0x64006400u), even);
+    }
     static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
         const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
         return *reinterpret_cast<const uint32_t*>(&d);
-    }
-    // (64 + q) twice: 64.0 is 0x5400, and a nibble on bits 4-7 of its ten-bit mantissa counts in ones; left shifts are
-    // multiplications (FMA pipe), so a word takes one shift and four LOP3
-    template <int I> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-        const uint32_t t = I < 2 ? w : w >> 8;
-        return and_or(I & 1 ? t : t * 16u, 0x00F000F0u, 0x54005400u);
     }
     // d = a * b + d, or a * b where FIRST (no registers to clear before a group's first step)
     template <bool FIRST>
@@ -373,9 +377,13 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
 #pragma unroll
                     for (int h = 0; h < 4; ++h) w[h] = *reinterpret_cast<const Words*>(words + 8 * h * (SLICE / 2));
                     float acc[2][4];
-                    uint32_t zr[4];
+                    uint32_t even[4], odd[4];   // base + z of the four rows
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) zr[h] = Z ? M::zero(zr_slice[h * 8 * 8 + p]) : M::EIGHT;
+                    for (int h = 0; h < 4; ++h) {
+                        const uint32_t z = Z ? zr_slice[h * 8 * 8 + p] : 8u;
+                        even[h] = M::template zero<0>(z);
+                        odd[h] = M::template zero<1>(z);
+                    }
 #pragma unroll
                     for (int st = 0; st < STEPS; ++st) {
                         const uint4 v = *reinterpret_cast<const uint4*>(here + x_row + (p * G + (c * STEPS + st) * 8) * 2);
@@ -384,13 +392,13 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
                             const uint32_t lo = w[2 * m].v[st], hi = w[2 * m + 1].v[st];
-                            const uint32_t zl = zr[2 * m], zh = zr[2 * m + 1];
-                            const uint32_t a0 = M::sub(M::template pair<0>(lo), zl), a1 = M::sub(M::template pair<0>(hi), zh);
-                            const uint32_t a2 = M::sub(M::template pair<1>(lo), zl), a3 = M::sub(M::template pair<1>(hi), zh);
+                            const uint32_t el = even[2 * m], eh = even[2 * m + 1], ol = odd[2 * m], oh = odd[2 * m + 1];
+                            const uint32_t a0 = M::template operand<0>(lo, el, ol), a1 = M::template operand<0>(hi, eh, oh);
+                            const uint32_t a2 = M::template operand<1>(lo, el, ol), a3 = M::template operand<1>(hi, eh, oh);
                             if (st == 0) M::template mma<true>(acc[m], a0, a1, a2, a3, b0, b1);
                             else M::template mma<false>(acc[m], a0, a1, a2, a3, b0, b1);
-                            M::template mma<false>(acc[m], M::sub(M::template pair<2>(lo), zl), M::sub(M::template pair<2>(hi), zh),
-                                                   M::sub(M::template pair<3>(lo), zl), M::sub(M::template pair<3>(hi), zh), b2, b3);
+                            M::template mma<false>(acc[m], M::template operand<2>(lo, el, ol), M::template operand<2>(hi, eh, oh),
+                                                   M::template operand<3>(lo, el, ol), M::template operand<3>(hi, eh, oh), b2, b3);
                         }
                     }
                     // C fragment: [0], [1] row g, columns 2c, 2c + 1; [2], [3] row g + 8.
@@ -425,7 +433,7 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
             const float* p = sums + col * RED_PITCH + row;
             float v = 0.f;
             for (int w = 0; w < a.split; ++w) v += p[w * layout.red_floats];
-            static_cast<T*>(a.out)[static_cast<size_t>(at.r0 + col) * a.ldo + at.n0 + row] = M::from_f32(v);
+            static_cast<T*>(a.out)[static_cast<size_t>(at.r0 + col) * a.ldo + at.n0 + row] = M::from_f32(v * M::UNIT);
         }
     }
     cp_async_wait_all();
