@@ -10,15 +10,15 @@
 //   * Nibbles become operands where they lie in a byte, two bytes at a time: by one AND or LOP3 and one packed FMA or
 //     subtraction that leaves q - z (bf16: times 2^-7), exactly; a word needs one shift.  So the products are exact and
 //     only the sums round, in fp32.  (One base for all nibbles takes three shifts and a multiplication, bf16, or one and
-//     two, fp16: 39 us at 16384 x 16384 where this takes 36 for both types; shifts as high halves of products 42 to 44; base and z
-//     taken off afterwards with sum x from one more MMA no less, and it costs bits.)
+//     two, fp16: with slices of 128, 39 us at 16384 x 16384 against 36; shifts as high halves of products 42 to 44; base and
+//     z taken off afterwards with sum x from one more MMA no less than 39, and it costs bits.)
 //   * A 32-bit word holds 8 consecutive k; the MMA's order of k is free as long as both operands follow it, so the
 //     pairs are (k, k + 4) as the masks deliver them, and x is brought into that order by four PRMTs per 8 values.
 //   * The four lanes of a quad take one, two or four consecutive words each, 32, 64 or 128 k together: a group, whose sum is
 //     then complete in the accumulator when its scale is applied (fp32).  A group of 128 is one 16-byte read per row.
-//   * A team of 1 to 16 warps takes 32 weight rows, each warp a range of k in slices of 128.  A slice (64 bytes of each
-//     weight row, 256 of each row of x) is two TMA copies into a ring of the warp's own, issued by one lane; the ring runs
-//     on across work items, so no barrier is between a copy and its use.  The copies' 64-byte swizzle keeps the reads free
+//   * A team of 1 to 16 warps takes 32 weight rows, each warp a range of k in slices of 128 or 256.  A slice (64 or 128
+//     bytes of each weight row, four times that of each row of x) is two TMA copies into a ring of the warp's own, issued by one lane; the ring runs
+//     on across work items, so no barrier is between a copy and its use.  The copies' swizzle keeps the reads free
 //     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
 //     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
 //   * The team's sums meet in shared memory once per item, added in warp order.
@@ -38,35 +38,45 @@ namespace w4 {
 constexpr int WARPS = 16;
 constexpr int ROWS = 32;                 // weight rows per item
 constexpr int THREADS = 32 * WARPS;
-constexpr int SLICE = 128;               // k per stage
 constexpr int COLS = 8;                  // rows of x per item: the columns of one MMA
-constexpr int X_PITCH = SLICE * 2;
-constexpr int W_BYTES = ROWS * SLICE / 2;
 constexpr int RED_PITCH = ROWS + 4;      // a fragment's 8 x 4 places lie in 32 banks
 constexpr int BLOCK = 8;                 // groups whose scales are copied at a time
 constexpr int SC_BYTES = ROWS * BLOCK * 3;   // a block: 16 bytes of scales per row, then 8 bytes of zero points per row
-constexpr int MAX_STAGES = 3;            // more only crowd the memory: copies alone of 16384 x 16384 take 25 us with three, 37 with six
 constexpr int MAX_EXPERTS = 1024;
 constexpr int SMEM_BYTES = 232448;
 
-// Shared memory: rings (512-byte aligned), scales (two blocks per warp), sums of the warps (two sets), barriers, flags, tables.
+// SLICE: k per stage.  256 halves what a slice costs besides its products; where one or two rows of x leave room for two
+// such stages per warp and k is long (launch_w4), 16384 x 16384 takes 33.4 us against 36.2, groups of 32 42.9 against 46.7.
+template <int SLICE>
+struct Cut {
+    static constexpr int X_PITCH = SLICE * 2;
+    static constexpr int W_BYTES = ROWS * SLICE / 2;
+    static constexpr int ALIGN = SLICE == 128 ? 512 : 1024;   // of a stage: the swizzle's period
+    static constexpr int MAX_STAGES = SLICE == 128 ? 3 : 2;   // more only crowd the memory: copies alone of 16384 x 16384 take
+                                                              // 25 us with three of 128, 37 with six
+};
+
+// Shared memory: rings, scales (two blocks per warp), sums of the warps (two sets), barriers, flags, tables.
+template <int SLICE>
 struct Layout {
     int xrows, stage, stages, red_floats, scales, red, bars, bytes;
     __host__ __device__ constexpr Layout(int rows, int experts)
         : xrows(0), stage(0), stages(0), red_floats(0), scales(0), red(0), bars(0), bytes(0) {
         xrows = rows < COLS ? rows : COLS;
-        stage = W_BYTES + (xrows * X_PITCH + 511) / 512 * 512;
+        using C = Cut<SLICE>;
+        stage = C::W_BYTES + (xrows * C::X_PITCH + C::ALIGN - 1) / C::ALIGN * C::ALIGN;
         red_floats = xrows * RED_PITCH;
-        const int rest = 1024 + WARPS * (2 * SC_BYTES + 2 * red_floats * 4 + MAX_STAGES * 8) + 16 + (experts > 1 ? (3 * experts + 1) * 4 : 16);
+        const int rest = 1024 + WARPS * (2 * SC_BYTES + 2 * red_floats * 4 + C::MAX_STAGES * 8) + 16 + (experts > 1 ? (3 * experts + 1) * 4 : 16);
         stages = (SMEM_BYTES - rest) / (WARPS * stage);
-        if (stages > MAX_STAGES) stages = MAX_STAGES;
+        if (stages > C::MAX_STAGES) stages = C::MAX_STAGES;
         scales = WARPS * stages * stage;
         red = scales + WARPS * 2 * SC_BYTES;
         bars = red + WARPS * 2 * red_floats * 4;
         bytes = rest + scales;
     }
 };
-static_assert(Layout(COLS, MAX_EXPERTS).stages >= 2, "a copy is in flight while a slice is used, at the largest sizes too");
+static_assert(Layout<128>(COLS, MAX_EXPERTS).stages >= 2 && Layout<256>(2, MAX_EXPERTS).stages >= 2,
+              "a copy is in flight while a slice is used, at the largest sizes too");
 }  // namespace w4
 
 // (a & b) | c in one instruction.
@@ -199,17 +209,18 @@ __device__ __forceinline__ void team_sync(int team, int threads) {
     if (threads > 32) asm volatile("barrier.cta.sync.aligned %0, %1;" ::"r"(team + 1), "r"(threads) : "memory");
 }
 
-template <typename T, int G, bool Z>
+template <typename T, int G, bool Z, int SLICE>
 __global__ void __launch_bounds__(w4::THREADS, 1)
 gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     using namespace w4;
     using M = W4Type<T>;
-    constexpr int PER = SLICE / G;          // groups per slice: 4, 2, 1
+    constexpr int X_PITCH = Cut<SLICE>::X_PITCH, W_BYTES = Cut<SLICE>::W_BYTES, MAX_STAGES = Cut<SLICE>::MAX_STAGES;
+    constexpr int PER = SLICE / G;          // groups per slice
     constexpr int STEPS = G / 32;           // steps per group, and consecutive words per lane
     constexpr int RUN = BLOCK / PER;        // slices per block of scales
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    const Layout layout(a.rows, a.experts);
+    const Layout<SLICE> layout(a.rows, a.experts);
     float* red = reinterpret_cast<float*>(smem + layout.red);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + layout.bars);
     uint32_t* flags = reinterpret_cast<uint32_t*>(bars + WARPS * MAX_STAGES);
@@ -335,7 +346,7 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
     uint32_t phase = 0;
     bool timed_out = false;
     // Where a lane reads in a stage: its words of row g (rows 8 apart have the same swizzle), its pieces of x.
-    const int w_row = g * (SLICE / 2), w_swizzle = (g >> 1) & 3;
+    const int w_row = g * (SLICE / 2), w_swizzle = SLICE == 128 ? (g >> 1) & 3 : g;   // of 64 or 128 bytes
     const int x_row = W_BYTES + min(g, layout.xrows - 1) * X_PITCH;   // columns without a row of x repeat one; they are not stored
     for (at.t = t_first; at.t < total; at.t += t_step) {
         at.decode(a, first, last, items);
@@ -448,15 +459,16 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-// Weights as bytes [experts][n][k / 2], boxes of 64 bytes x 32 rows; x as rows of 16-bit elements, boxes of 128 x xrows.
-int w4_maps(CUtensorMap* map_w, CUtensorMap* map_x, const W4Args& a, const uint8_t* q, const void* x, long long ldx, int xrows) {
+// Weights as bytes [experts][n][k / 2], boxes of a slice of 32 rows; x as rows of 16-bit elements, boxes of a slice of xrows.
+int w4_maps(CUtensorMap* map_w, CUtensorMap* map_x, const W4Args& a, const uint8_t* q, const void* x, long long ldx, int xrows, int slice) {
     const cuuint64_t wdims[3] = {static_cast<cuuint64_t>(a.k) / 2, static_cast<cuuint64_t>(a.n), static_cast<cuuint64_t>(a.experts)};
     const cuuint64_t wstrides[2] = {static_cast<cuuint64_t>(a.k) / 2, static_cast<cuuint64_t>(a.n) * a.k / 2};
-    const cuuint32_t wbox[3] = {w4::SLICE / 2, w4::ROWS, 1};
-    if (int rc = encode_tensor_map(map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, q, wdims, wstrides, wbox, CU_TENSOR_MAP_SWIZZLE_64B)) return rc;
+    const cuuint32_t wbox[3] = {static_cast<cuuint32_t>(slice) / 2, w4::ROWS, 1};
+    if (int rc = encode_tensor_map(map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, q, wdims, wstrides, wbox,
+                                    slice == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     const cuuint64_t xdims[2] = {static_cast<cuuint64_t>(a.k), static_cast<cuuint64_t>(a.rows)};
     const cuuint64_t xstrides[1] = {static_cast<cuuint64_t>(ldx) * 2};
-    const cuuint32_t xbox[2] = {w4::SLICE, static_cast<cuuint32_t>(xrows)};
+    const cuuint32_t xbox[2] = {static_cast<cuuint32_t>(slice), static_cast<cuuint32_t>(xrows)};
     return encode_tensor_map(map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, x, xdims, xstrides, xbox, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
@@ -468,8 +480,8 @@ long long most_items(const W4Args& a) {
 }
 
 // Warps per team: the fewest rounds of (slices per warp + the item's own cost, about one slice) over all teams.
-int w4_split(const W4Args& a, int sms) {
-    const int slices = (a.k + w4::SLICE - 1) / w4::SLICE;
+int w4_split(const W4Args& a, int sms, int slice) {
+    const int slices = (a.k + slice - 1) / slice;
     long long least = 0;
     int best = 1;
     for (int split = 1; split <= w4::WARPS && (split == 1 || split <= slices); split *= 2) {
@@ -483,9 +495,9 @@ int w4_split(const W4Args& a, int sms) {
     return best;
 }
 
-template <typename T, int G, bool Z>
+template <typename T, int G, bool Z, int SLICE>
 int launch_w4(W4Args a, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
-    auto kern = gemv_w4_kernel<T, G, Z>;
+    auto kern = gemv_w4_kernel<T, G, Z, SLICE>;
     static std::mutex mu;
     static int sm_count[64] = {};
     int dev = 0, sms = 0;
@@ -501,10 +513,10 @@ int launch_w4(W4Args a, const uint8_t* q, const void* x, long long ldx, cudaStre
             sms = sm_count[dev];
         }
     }
-    a.split = w4_split(a, sms);
-    const w4::Layout layout(a.rows, a.experts);
+    a.split = w4_split(a, sms, SLICE);
+    const w4::Layout<SLICE> layout(a.rows, a.experts);
     CUtensorMap map_w, map_x;
-    if (int rc = w4_maps(&map_w, &map_x, a, q, x, ldx, layout.xrows)) return rc;
+    if (int rc = w4_maps(&map_w, &map_x, a, q, x, ldx, layout.xrows, SLICE)) return rc;
     const int teams = w4::WARPS / a.split;
     const long long blocks = (most_items(a) + teams - 1) / teams;
     kern<<<static_cast<int>(blocks < sms ? blocks : sms), w4::THREADS, layout.bytes, s>>>(a, map_w, map_x);
@@ -513,9 +525,15 @@ int launch_w4(W4Args a, const uint8_t* q, const void* x, long long ldx, cudaStre
     return PRISM_B200_OK;
 }
 
+template <typename T, int G, bool Z>
+int launch_w4_slice(const W4Args& a, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
+    // Below 4096 the longer slices are too few to go round (2048 x 1024: 4.8 us against 4.2; 4096 x 4096: 5.2 against 5.3).
+    return a.rows <= 2 && a.k >= 4096 ? launch_w4<T, G, Z, 256>(a, q, x, ldx, s) : launch_w4<T, G, Z, 128>(a, q, x, ldx, s);
+}
+
 template <typename T, int G>
 int launch_w4_zeros(const W4Args& a, const uint8_t* q, const void* x, long long ldx, cudaStream_t s) {
-    return a.zeros ? launch_w4<T, G, true>(a, q, x, ldx, s) : launch_w4<T, G, false>(a, q, x, ldx, s);
+    return a.zeros ? launch_w4_slice<T, G, true>(a, q, x, ldx, s) : launch_w4_slice<T, G, false>(a, q, x, ldx, s);
 }
 
 template <typename T>

@@ -74,6 +74,19 @@ def test_k_that_ends_inside_a_slice(pb, dtype, zeros):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_one_or_two_rows_of_long_k(pb, dtype, zeros, group):
+    """Slices of 256 k: ends inside one, with and without whole blocks of eight scales, one matrix or several."""
+    for n, k in ((70, 4096), (33, 4096 + group), (200, 4096 + 3 * group), (5000, 4224), (8, 12288)):
+        for rows in (1, 2):
+            check(pb, [rows], 0, n, k, group, dtype, zeros, seed=k, exact=True, grouped=False)
+            check(pb, [rows], 0, n, k, group, dtype, zeros, seed=n, grouped=False)
+    check(pb, [0, 1, 0, 1], 0, 96, 4096, group, dtype, zeros, seed=5, exact=True)
+    check(pb, [0, 1], 1, 96, 4352, group, dtype, zeros, seed=6)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("group", [32, 128])
 def test_groups_of_rows(pb, dtype, group):
     for sizes, spare in (([1], 0), ([0, 3, 0], 2), ([8, 9, 1, 0, 16, 17], 0), ([1] * 40, 5), ([0, 0], 1), ([60, 0, 4], 0)):
