@@ -203,6 +203,16 @@ struct Item {
     }
 };
 
+// The weight row (of eight) that takes place g of the MMA's fragments: the order in which lanes that read together find
+// their pieces in different banks.  A slice's rows lie 64 or 128 bytes apart, 16-byte pieces XORed by the row.
+template <int SLICE, int G>
+__device__ __forceinline__ int fragment_row(int g) {
+    if (SLICE == 256 && G == 128) return g >> 1 | (g & 1) << 2;
+    if (SLICE == 256 && G == 64) return (g & 3) << 1 | g >> 2;
+    if (SLICE == 128 && G == 64) return (g & 1) | (g & 2) << 1 | (g & 4) >> 1;
+    return g;
+}
+
 // Barrier of the warps of team `team` (named barrier team + 1).
 __device__ __forceinline__ void team_sync(int team, int threads) {
     __syncwarp();
@@ -345,8 +355,9 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
     int slot = 0, set = 0, block = 0;
     uint32_t phase = 0;
     bool timed_out = false;
-    // Where a lane reads in a stage: its words of row g (rows 8 apart have the same swizzle), its pieces of x.
-    const int w_row = g * (SLICE / 2), w_swizzle = SLICE == 128 ? (g >> 1) & 3 : g;   // of 64 or 128 bytes
+    // Where a lane reads in a stage: its words of row wr (rows 8 apart have the same swizzle), its pieces of x.
+    const int wr = fragment_row<SLICE, G>(g);
+    const int w_row = wr * (SLICE / 2), w_swizzle = SLICE == 128 ? (wr >> 1) & 3 : wr;   // of 64 or 128 bytes
     const int x_row = W_BYTES + min(g, layout.xrows - 1) * X_PITCH;   // columns without a row of x repeat one; they are not stored
     for (at.t = t_first; at.t < total; at.t += t_step) {
         at.decode(a, first, last, items);
@@ -376,11 +387,11 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
                     slot = 0;
                     phase ^= 1u;
                 }
-                const unsigned char* sc_slice = sc_block + g * 16 + (s % RUN) * (PER * 2);
-                const unsigned char* zr_slice = sc_block + ROWS * 16 + g * 8 + (s % RUN) * PER;
+                const unsigned char* sc_slice = sc_block + wr * 16 + (s % RUN) * (PER * 2);
+                const unsigned char* zr_slice = sc_block + ROWS * 16 + wr * 8 + (s % RUN) * PER;
 #pragma unroll
                 for (int p = 0; p < PER; ++p) {
-                    // A lane's STEPS consecutive words in rows g, g + 8, g + 16, g + 24.
+                    // A lane's STEPS consecutive words in rows wr, wr + 8, wr + 16, wr + 24.
                     struct alignas(4 * STEPS) Words { uint32_t v[STEPS]; };
                     Words w[4];
                     const int byte = p * (G / 2) + c * (4 * STEPS);   // in the row's 64
@@ -412,7 +423,7 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
                                                    M::template operand<3>(lo, el, ol), M::template operand<3>(hi, eh, oh), b2, b3);
                         }
                     }
-                    // C fragment: [0], [1] row g, columns 2c, 2c + 1; [2], [3] row g + 8.
+                    // C fragment: [0], [1] row wr, columns 2c, 2c + 1; [2], [3] row wr + 8.
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         const float sc = M::to_f32(*reinterpret_cast<const uint16_t*>(sc_slice + h * 8 * 16 + p * 2));
@@ -435,7 +446,7 @@ gemv_w4_kernel(const W4Args a, const __grid_constant__ CUtensorMap map_w, const 
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int col = 2 * c + (i & 1);
-                if (col < cols) part[col * RED_PITCH + m * 16 + (i >> 1) * 8 + g] = sum[m][i];
+                if (col < cols) part[col * RED_PITCH + m * 16 + (i >> 1) * 8 + wr] = sum[m][i];
             }
         team_sync(team, team_threads);
         for (int i = warp_k * 32 + lane; i < cols * ROWS; i += team_threads) {
