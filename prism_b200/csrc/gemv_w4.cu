@@ -22,9 +22,9 @@
 //     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
 //     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
 //   * The team's sums meet in shared memory once per item, added in warp order.
-// Where the time goes: 16384 x 16384, one row, takes 36 us; the copies alone take 25.  On the SMs at work the schedulers
-// issue in 70% of the cycles and the ALU pipe is 66% busy; the tensor pipe, an mma.sync taking it 8 cycles per scheduler,
-// is at 30%.  512 tiles in teams of four warps use 128 of the 148 SMs: 18944 rows, which use all, take 37 us (4.3 TB/s).
+// Where the time goes: 16384 x 16384, one row, takes 32.5 us; the copies alone take 25.  On the SMs at work the schedulers
+// issue in 69% of the cycles and the ALU pipe is 64% busy; the tensor pipe, an mma.sync taking it 8 cycles per scheduler,
+// is at 33%.  512 tiles in teams of four warps use 128 of the 148 SMs: 18944 rows, which use all, take 33.2 us (4.8 TB/s).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
