@@ -17,10 +17,10 @@
 //   * The four lanes of a quad take one, two or four consecutive words each, 32, 64 or 128 k together: a group, whose sum is
 //     then complete in the accumulator when its scale is applied (fp32).  A group of 128 is one 16-byte read per row.
 //   * A team of 1 to 16 warps takes 32 weight rows, each warp a range of k in slices of 128 or 256.  A slice (64 or 128
-//     bytes of each weight row, four times that of each row of x) is two TMA copies into a ring of the warp's own, issued by one lane; the ring runs
-//     on across work items, so no barrier is between a copy and its use.  The copies' swizzle keeps the reads free
-//     of bank conflicts, and what lies outside the matrices arrives as zeros.  Scales and zero points come in blocks of
-//     eight groups (16 and 8 bytes per row, cp.async) one block ahead.
+//     bytes of each weight row, four times that of each row of x) is two TMA copies into a ring of the warp's own, issued
+//     by one lane; the ring runs on across work items, so no barrier is between a copy and its use.  What lies outside the
+//     matrices arrives as zeros.  The copies' swizzle and the order of the fragments' rows keep the reads free of bank
+//     conflicts.  Scales and zero points come in blocks of eight groups (16 and 8 bytes per row, cp.async) one block ahead.
 //   * The team's sums meet in shared memory once per item, added in warp order.
 // Where the time goes: 16384 x 16384, one row, takes 32.5 us; the copies alone take 25.  On the SMs at work the schedulers
 // issue in 69% of the cycles and the ALU pipe is 64% busy; the tensor pipe, an mma.sync taking it 8 cycles per scheduler,

@@ -190,3 +190,29 @@ def test_rows_past_32_bits(pb):
     assert torch.equal(dy[at], (weights[:, :, None] * x[:, None].float()).to(BF))
     assert torch.equal(dweights, (y[at].double() * x[:, None].double()).sum(2).float())
     assert bool((dy[50:rows - T * k + 50] == 7.0).all())
+
+
+def test_threads_on_streams_of_their_own(pb):
+    """Four host threads at once: each one's results repeat bit for bit and no call fails."""
+    import threading
+    wrong = []
+
+    def work(seed):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for T in (1, 60, 130, 900):
+                    logits, x, w1, w2, dout = make(T, 16, 3, 128, 192, seed=seed + T)
+                    a, r = layer(pb, logits, x, w1, w2, dout, 3)
+                    b, _ = layer(pb, logits, x, w1, w2, dout, 3)
+                    wrong.extend((seed, T, name) for name in a if not torch.equal(a[name], b[name]))
+            stream.synchronize()
+        except Exception as e:  # noqa: BLE001 -- reported by the test's own thread
+            wrong.append((seed, repr(e)))
+
+    threads = [threading.Thread(target=work, args=(100 * i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and pb.last_error()[0] == 0
