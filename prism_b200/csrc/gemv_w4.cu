@@ -91,6 +91,7 @@ template <> struct W4Type<__nv_bfloat16> {
     static constexpr float UNIT = 128.f;   // operands are (q - z) / 128
     // An integer in the lowest eight bits of a bf16 is itself times 2^-133, through the subnormals and the first normal
     // numbers; so both nibbles of a byte serve where they lie, and one FMA scales them and takes z off, exactly.
+    // (Products with subnormal x stay exact too: 2^-133 / 128 is 2^-140, and fp32 goes down to 2^-149.)
     template <int ODD> static __device__ __forceinline__ uint32_t zero(uint32_t z) { return ODD ? 0u : fma(z * 0x10001u, 0xFE80FE80u, 0u); }
     template <int I> static __device__ __forceinline__ uint32_t operand(uint32_t w, uint32_t even, uint32_t odd) {
         const uint32_t s = I < 2 ? w : w >> 8;

@@ -131,6 +131,21 @@ def test_a_nan_stays_in_its_row(pb):
     assert torch.equal(clean[keep], dirty[keep]) and not torch.isfinite(dirty[[4, 10]]).any()
 
 
+@pytest.mark.parametrize("dtype,exponents", [(BF, (120, 100, -100, -119, -120, -126, -130, -133)), (HF, (10, -14, -20, -24))])
+def test_the_smallest_and_largest_values(pb, dtype, exponents):
+    """x near the ends of its type, subnormals included: products and sums of equal powers of two are exact."""
+    k, n = 4096, 40
+    q = torch.full((n, k // 2), 0x99, dtype=torch.uint8, device=DEV)   # 9 - 8
+    for e in exponents:
+        scale = 100 if e < -60 else 8 if e < 0 else -30 if e > 60 else -14
+        x = torch.full((2, k), 2.0 ** e, dtype=torch.float64, device=DEV).to(dtype)
+        x[1, 1::2] = 0
+        scales = torch.full((n, k // 128), 2.0 ** scale, dtype=torch.float64, device=DEV).to(dtype)
+        for rows in (x, x.repeat(4, 1)):
+            got = pb.gemv_w4(rows, q, scales)[:2].double()
+            assert bool((got[0] == k * 2.0 ** (e + scale)).all() and (got[1] == k * 2.0 ** (e + scale - 1)).all()), e
+
+
 def test_graph_and_streams(pb):
     q, scales, z = weights((3,), 96, 384, 128, BF, True, 10)
     x, offsets = torch.randn((10, 384), device=DEV).to(BF), borders([4, 0, 6])
